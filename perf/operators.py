@@ -214,6 +214,16 @@ def prepare(case, seed):
     return s
 
 
+class _Owned:
+    """A buffer that lives as long as somebody holds a view of it."""
+
+    def __init__(self, rt, i):
+        self.rt, self.id = rt, i
+
+    def __del__(self):
+        self.rt.release_buffers([self.id], 1)
+
+
 class _Handle:
     """What a program built on the framework keeps: its device buffers, the cache object and the recorded streams."""
 
@@ -221,22 +231,22 @@ class _Handle:
         from deepj_b200 import _lib
         from deepj_b200 import compute_graph as cg
         self.rt = cg.CudaGpuRuntime()
-        self.lib, self.ids = self.rt.lib, []
+        self.lib, self.ids, self.views = self.rt.lib, [], []
         case = s["case"]
         batch, groups, dim, size, history = case["batch"], case["groups"], case["dim"], s["size"], k.shape[2]
-        kv = self._id()
+        kv = self._object()
         _lib.check(self.lib.deepj_cuda_kv_alloc_q4(kv, 1, batch, groups, size, dim))
         rows, view = self._buffer(batch * history, 2 * groups * dim)
         at, _ = self._buffer(batch)
         view.view(batch, history, 2, groups, dim).copy_(torch.stack((k, v), 2).permute(0, 3, 2, 1, 4))
         torch.cuda.synchronize()
         self._flush([cg.OP_KV_STORE_Q4, rows, 0, groups * dim, 2 * groups * dim, kv, 0, at, batch, history])
-        self.rt.release_buffers([rows], 1)
-        self.ids.remove(rows)
+        self.views.pop(0)                        # the rows are in the cache: their buffer goes
+        del view
         length, acc = self._given(s["len"]), self._given(s["weights"])
         if case["op"] == "evict":
             keep = case["budget"]
-            small = self._id()
+            small = self._object()
             _lib.check(self.lib.deepj_cuda_kv_alloc_q4(small, 1, batch, groups, keep, dim))
             acc_out, acc_view = self._buffer(batch, groups, keep)
             len_out, len_view = self._buffer(batch)
@@ -270,15 +280,20 @@ class _Handle:
         self.stream = cg.stream(stream)
         torch.cuda.synchronize()
 
-    def _id(self):
+    def _object(self):
         _next_id[0] += 1
         self.ids.append(_next_id[0])
         return _next_id[0]
 
     def _buffer(self, *shape):
-        i, n = self._id(), math.prod(shape)
-        self.rt.alloc_buffers([i], [n], 1)
-        return i, torch.as_tensor(self.rt.device_view(i, shape), device="cuda")
+        _next_id[0] += 1
+        i = _next_id[0]
+        self.rt.alloc_buffers([i], [math.prod(shape)], 1)
+        self.rt.synchronize()                    # its zeros are written before torch's stream writes into it
+        seen = self.rt.device_view(i, shape)
+        seen.owner = _Owned(self.rt, i)          # the tensor keeps what it was made from, and that keeps the buffer
+        self.views.append(torch.as_tensor(seen, device="cuda"))
+        return i, self.views[-1]
 
     def _given(self, x):
         i, view = self._buffer(*x.shape)
