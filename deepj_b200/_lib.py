@@ -42,6 +42,8 @@ SIGNATURES = {
     "deepj_cuda_synth_fill": (ctypes.c_int, [ctypes.c_int32, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_float, ctypes.c_int64, ctypes.c_int64]),
     "deepj_cuda_kv_alloc": (ctypes.c_int, [ctypes.c_int32] * 6),
     "deepj_cuda_kv_alloc_f16": (ctypes.c_int, [ctypes.c_int32] * 6),
+    "deepj_cuda_kv_alloc_q4": (ctypes.c_int, [ctypes.c_int32] * 6),
+    "deepj_cuda_buffer_address": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64), _i64p]),
     "deepj_cuda_bf16_alloc": (ctypes.c_int, [ctypes.c_int32] * 3),
     "deepj_cuda_bf16_store": (ctypes.c_int, [ctypes.c_int32] * 5 + [ctypes.c_int64] + [ctypes.c_int32] * 2),
     "deepj_cuda_latent_alloc": (ctypes.c_int, [ctypes.c_int32] * 5),

@@ -37,6 +37,7 @@ OP_ATTN_PREFILL, OP_SAMPLE_TOPK, OP_Q8_LINEAR_LN, OP_DECODE_STEP = 73, 74, 75, 7
 # ops over bf16 weights
 OP_BF16_LINEAR, OP_BF16_BLOCK_LINEAR, OP_DELTA_RULE, OP_ATTN_LATENT, OP_TABLE_EXPERTS = 77, 78, 79, 80, 81
 OP_ATTN_LATENT_CHUNK, OP_BF16_LINEAR_SUM, OP_NORM_ADD, OP_ATTN_GROUPED, OP_MLSTM = 82, 83, 84, 85, 86
+OP_ATTN_DECODE_Q4, OP_ATTN_PACKED_Q4, OP_KV_EVICT_Q4, OP_KV_STORE_Q4, OP_KV_LOAD_Q4 = 87, 88, 89, 90, 91
 
 # op → (stride, offsets of the slots that hold buffer ids); ComputeGraph.java:89-147
 OP_METADATA: Dict[int, tuple] = {}
@@ -82,12 +83,22 @@ OP_METADATA[OP_BF16_LINEAR_SUM] = (38, (1, 4, 7, 11, 14, 15, 18, 24, 29, 31, 35)
 OP_METADATA[OP_NORM_ADD] = (13, (1, 4, 6, 10))
 OP_METADATA[OP_ATTN_GROUPED] = (27, (1, 6, 7, 9, 10, 12, 13, 14, 15, 16))
 OP_METADATA[OP_MLSTM] = (22, (1, 10, 11, 12, 13))
+OP_METADATA[OP_ATTN_DECODE_Q4] = (20, (1, 6, 8, 9, 10, 11, 13, 18, 19))
+OP_METADATA[OP_ATTN_PACKED_Q4] = (23, (1, 6, 8, 9, 10, 11, 12, 14, 20, 21))
+OP_METADATA[OP_KV_EVICT_Q4] = (12, (1, 2, 4, 5, 9, 10, 11))
+OP_METADATA[OP_KV_STORE_Q4] = (10, (1, 5, 7))
+OP_METADATA[OP_KV_LOAD_Q4] = (9, (1, 3, 4, 6, 7))
 
 
 def float_bits(value: float) -> int:
     """Float.floatToRawIntBits: the int32 that carries a float through the stream
     (ComputeGraph.java:252-254)."""
     return struct.unpack("<i", struct.pack("<f", float(np.float32(value))))[0]
+
+
+def stream(words: Sequence[int]) -> np.ndarray:
+    """Op words as the int32 stream that a flush takes."""
+    return np.asarray([int(w) for w in words], dtype=np.int32)
 
 
 class GpuRuntime(Protocol):
@@ -127,6 +138,31 @@ class CudaGpuRuntime:
     def flush_ops(self, cmd_stream, length):
         cmd = np.ascontiguousarray(cmd_stream[:length], dtype=np.int32)
         _lib.check(self.lib.deepj_cuda_flush_ops(cmd.ctypes.data, length))
+
+    def flush_ops_async(self, cmd_stream, length):
+        """The same, enqueued: results are there after `synchronize` (or any call that waits for the device)."""
+        cmd = np.ascontiguousarray(cmd_stream[:length], dtype=np.int32)
+        _lib.check(self.lib.deepj_cuda_flush_ops_async(cmd.ctypes.data, length))
+
+    def synchronize(self):
+        _lib.check(self.lib.deepj_cuda_synchronize())
+
+    def device_view(self, buf_id: int, shape: Sequence[int]) -> "DeviceView":
+        """A float buffer's device memory as `__cuda_array_interface__`, for libraries that share the device: no copy is made, work on
+        other streams is the caller's to order (`synchronize`), and the view ends with the buffer."""
+        address, floats = ctypes.c_uint64(), ctypes.c_int64()
+        _lib.check(self.lib.deepj_cuda_buffer_address(buf_id, ctypes.byref(address), ctypes.byref(floats)))
+        need = 1
+        for n in shape:
+            need *= int(n)
+        if any(int(n) < 0 for n in shape) or need > floats.value:
+            raise ValueError(f"buffer id={buf_id} holds {floats.value} floats, the view needs {need}")
+        return DeviceView(address.value, tuple(int(n) for n in shape))
+
+
+class DeviceView:
+    def __init__(self, address: int, shape: tuple):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": "<f4", "data": (address, False), "strides": None, "version": 3}
 
 
 class GpuBuffer:

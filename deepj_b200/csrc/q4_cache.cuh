@@ -1,0 +1,63 @@
+// The 4-bit K/V cache: its layout in memory and the quantization of a row, shared by the kernels that fill it, read it and move its rows.
+//
+// A row (the key or the value of one position and key/value head) of hd = 32·NB values is NB blocks of 32: a bf16 scale
+//     s = bf16(max|w| · fp32(1/7)), at least 2^-17 and at most 2^13; 0 where the block is all zeros
+// and 32 codes clamp(round_half_even(w / s), -7, 7), NaN → 0.  A code has 3 bits and a sign, s has 8 bits: code · s is exact in fp16 over the whole
+// range of s, which is what lets the tensor cores multiply stored values without a correction term.
+// Rows lie in pages of 32 consecutive positions, 1152·NB contiguous bytes that one bulk copy brings:
+//     K codes [32][16·NB] | V codes [32][16·NB] | K scales [32][NB] bf16 | V scales [32][NB] bf16
+// Word (t, j) of a row, t < 4, j < NB, holds as nibbles code + 8: byte i the dims 32j + 4t + i (low) and 32j + 16 + 4t + i (high), so that masking
+// a word gives two operand registers of m16n8k32.  The words of one t are a piece of 4·NB bytes; piece t of row r sits in slot t ^ (r/2 % 4): with
+// rows of 64 bytes the warp that reads one piece of four consecutive rows finds them in different banks.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "q8_common.cuh"
+
+namespace dj {
+
+constexpr int kQ4Page = 32;
+constexpr int kQ4PageBytes = 1152;               // … times NB
+constexpr float kQ4ScaleMin = 1.0f / 131072.0f, kQ4ScaleMax = 8192.0f;
+
+template <int NB> struct Q4Page {
+    static constexpr int kBytes = kQ4PageBytes * NB, kRow = 16 * NB;
+    static constexpr int kV = kQ4Page * kRow, kKs = 2 * kV, kVs = kKs + kQ4Page * NB * 2;      // offsets of the V codes and of the scales
+    static __device__ __forceinline__ int word(int row, int t, int j) { return row * kRow + (t ^ ((row >> 1) & 3)) * (4 * NB) + 4 * j; }
+};
+
+// Rows that a sequence has room for and positions that its tables have, of `tokens` new ones: 0 for a length or position outside its range.
+__device__ __forceinline__ int q4_room(int tokens, int len, int maxSeq, int pos, int maxPos) {
+    if (len < 0 || len >= maxSeq || pos < 0 || pos >= maxPos) return 0;
+    return max(0, min(tokens, min(maxSeq - len, maxPos - pos)));
+}
+
+// The eight lanes of a block hold four values each → the block's scale and this lane's four codes + 8 in the low nibbles of a word's bytes.
+__device__ __forceinline__ uint32_t q4_codes(float4 x, float& scale) {
+    x.x = x.x == x.x ? x.x : 0.0f; x.y = x.y == x.y ? x.y : 0.0f; x.z = x.z == x.z ? x.z : 0.0f; x.w = x.w == x.w ? x.w : 0.0f;
+    float most = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const float s = fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(most * (1.0f / 7.0f))), kQ4ScaleMin), kQ4ScaleMax);
+    scale = most > 0.0f ? s : 0.0f;
+    auto code = [&](float v) { return (uint32_t)((int)fminf(fmaxf(rintf(v / s), -7.0f), 7.0f) + 8); };
+    return code(x.x) | code(x.y) << 8 | code(x.z) << 16 | code(x.w) << 24;
+}
+
+// 8·NB consecutive lanes (all lanes of the warp are here) put one row into its page: lane e of them holds the values 4e … 4e + 3.
+template <int NB>
+__device__ __forceinline__ void q4_put_row(unsigned char* page, int row, bool value, int e, const float4& x, bool on) {
+    float scale;
+    const uint32_t mine = q4_codes(x, scale), other = __shfl_xor_sync(0xffffffffu, mine, 4);
+    if (!on) return;
+    const int j = e >> 3, t = e & 3;
+    if ((e & 4) == 0) *reinterpret_cast<uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(row, t, j)) = mine | other << 4;
+    if ((e & 7) == 0) *reinterpret_cast<__nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (row * NB + j) * 2) = __float2bfloat16_rn(scale);
+}
+
+// interleaved pairs (x0, x1) → (x0·c − x1·s, x0·s + x1·c), every product and sum rounded (RotaryEmbedding.java:81-122)
+__device__ __forceinline__ float4 q4_rotate(const float4& x, const float2& c, const float2& s) {
+    return make_float4(x.x * c.x - x.y * s.x, x.x * s.x + x.y * c.x, x.z * c.y - x.w * s.y, x.z * s.y + x.w * c.y);
+}
+
+}  // namespace dj

@@ -59,14 +59,14 @@ using namespace dj;
 
 thread_local std::string g_err;
 
-enum BufKind { kF32 = 0, kQ8 = 1, kKV = 2, kPlan = 3, kBf16 = 4, kLatent = 5 };
+enum BufKind { kF32 = 0, kQ8 = 1, kKV = 2, kPlan = 3, kBf16 = 4, kLatent = 5, kQ4 = 6 };
 struct Buf {
     BufKind kind = kF32;
     void* ptr = nullptr;
     size_t bytes = 0;
     size_t floats = 0;                 // kF32
     int K = 0, N = 0, Kp = 0, nb = 0;  // kQ8, kBf16
-    int layers = 0, B = 0, H = 0, maxSeq = 0, hd = 0, kvHalf = 0;   // kKV (kvHalf: fp16 elements), kLatent (B, maxSeq, hd = row width; kvHalf: bf16 elements)
+    int layers = 0, B = 0, H = 0, maxSeq = 0, hd = 0, kvHalf = 0;   // kKV (kvHalf: fp16 elements), kQ4 (H: key/value heads), kLatent (B, maxSeq, hd = row width; kvHalf: bf16 elements)
     unsigned long long serial = 0;
 };
 
@@ -270,6 +270,7 @@ void check_part(int op) {
     else if (op == DEEPJ_OP_ATTN_DECODE || op == DEEPJ_OP_ATTN_PREFILL) part(launch_attn_decode, "attention");
     else if (op == DEEPJ_OP_TP_ALLREDUCE || op == DEEPJ_OP_TP_ALLGATHER) part(launch_tp_exchange, "tensor-parallel exchange");
     else if (op == DEEPJ_OP_DECODE_STEP) part(launch_decode_step, "whole-token kernel");
+    else if (op >= DEEPJ_OP_ATTN_DECODE_Q4) part(launch_q4_attn, "4-bit cache");
     else if (op >= DEEPJ_OP_BF16_LINEAR) part(launch_bf16_linear, "bf16 projections and their mixers");
 }
 
@@ -305,11 +306,23 @@ int op_stride(int op) {
         case DEEPJ_OP_NORM_ADD: return 13;
         case DEEPJ_OP_ATTN_GROUPED: return 27;
         case DEEPJ_OP_MLSTM: return 22;
+        case DEEPJ_OP_ATTN_DECODE_Q4: return 20;
+        case DEEPJ_OP_ATTN_PACKED_Q4: return 23;
+        case DEEPJ_OP_KV_EVICT_Q4: return 12;
+        case DEEPJ_OP_KV_STORE_Q4: return 10;
+        case DEEPJ_OP_KV_LOAD_Q4: return 9;
         default: return -1;
     }
 }
 
 inline size_t sz(int a, int b) { return (size_t)a * (size_t)b; }
+
+// A layer of a 4-bit cache that at least B sequences fit into.
+unsigned char* q4_layer(const Buf& kv, int B, int layer, const char* what) {
+    require(B >= 1 && B <= kv.B, what, "batch does not match the cache");
+    require(layer >= 0 && layer < kv.layers, what, "layer out of range");
+    return (unsigned char*)kv.ptr + (size_t)layer * q4_plane_bytes(kv.B, kv.H, kv.maxSeq, kv.hd);
+}
 
 // Decode one op at c; validate; launch when ctx.execute.
 void do_op(Ctx& ctx, const int32_t* c) {
@@ -713,6 +726,90 @@ void do_op(Ctx& ctx, const int32_t* c) {
             a.early = early;
             a.ws = scratch(mlstm_ws_floats(a));
             if (go) launch_mlstm(a, s);
+            break;
+        }
+        case DEEPJ_OP_ATTN_DECODE_Q4:
+        case DEEPJ_OP_ATTN_PACKED_Q4: {
+            // 87: [op, qkv, q_off, k_off, v_off, ld, kv, layer, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, acc, acc_out]
+            // 88: [op, qkv, q_off, k_off, v_off, ld, kv, layer, starts, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, M, acc, acc_out, window]
+            const bool packed = op == DEEPJ_OP_ATTN_PACKED_Q4;
+            const char* what = packed ? "attnPackedQ4" : "attnDecodeQ4";
+            const int32_t* e = packed ? c + 1 : c;          // fields from len on sit one slot later in op 88
+            const int32_t* w = packed ? c + 20 : c + 18;    // acc, acc_out
+            Buf& kv = find_buf(ctx, c[6], kQ4, what);
+            Q4AttnArgs a = {};
+            a.B = e[16]; a.H = e[17]; a.G = kv.H; a.hd = kv.hd; a.maxSeq = kv.maxSeq; a.maxPos = e[12];
+            a.cache = q4_layer(kv, a.B, c[7], what);
+            a.M = packed ? c[19] : a.B; a.window = packed ? c[22] : 1;
+            require(a.M >= 0 && a.window >= 0 && a.maxPos >= 1, what, "bad dimension");
+            require(a.H >= 1 && a.H % a.G == 0 && a.H / a.G <= 64, what, "query heads must be a multiple (at most 64 times) of the cache's heads");
+            require((long long)a.H * a.hd <= 1 << 20 && a.G <= 65535, what, "too many heads");
+            a.q_off = c[2]; a.k_off = c[3]; a.v_off = c[4]; a.ld = c[5];
+            require(a.q_off >= 0 && a.k_off >= 0 && a.v_off >= 0 && e[14] >= 0, what, "negative offset");
+            require(a.ld % 4 == 0 && a.q_off % 4 == 0 && a.k_off % 4 == 0 && a.v_off % 4 == 0 && e[14] % 4 == 0 && e[15] % 4 == 0, what,
+                    "offsets and strides must be multiples of 4 floats");
+            const long long width = std::max((long long)a.q_off + a.H * a.hd, (long long)std::max(a.k_off, a.v_off) + a.G * a.hd);
+            require(a.ld >= width && e[15] >= a.H * a.hd, what, "row stride smaller than the row");
+            a.ldo = e[15];
+            const int last = std::max(a.M, 1) - 1;
+            a.qkv = f32(ctx, c[1], a.M ? sz(last, a.ld) + width : 0, what);
+            if (packed) a.starts = f32(ctx, c[8], (size_t)a.B + 1, what);
+            a.len = f32(ctx, e[8], a.B, what); a.pos = f32(ctx, e[9], a.B, what);
+            a.cosT = f32(ctx, e[10], sz(a.maxPos, a.hd / 2), what); a.sinT = f32(ctx, e[11], sz(a.maxPos, a.hd / 2), what);
+            a.out = f32(ctx, e[13], a.M ? (size_t)e[14] + sz(last, a.ldo) + a.H * a.hd : 0, what) + e[14];
+            require((w[0] < 0) == (w[1] < 0), what, "accumulated weights need both an input and an output (which may be the same buffer)");
+            require(!packed || (w[0] < 0) == (a.window == 0), what, "a window goes with accumulated weights, and they with a window");
+            a.acc = f32_opt(ctx, w[0], sz(a.B, a.G) * a.maxSeq, what); a.accOut = f32_opt(ctx, w[1], sz(a.B, a.G) * a.maxSeq, what);
+            a.tickets = R.tickets;
+            a.ws = scratch(q4_attn_ws_floats(a));
+            if (go) launch_q4_attn(a, s);
+            break;
+        }
+        case DEEPJ_OP_KV_EVICT_Q4: {   // [op, kv, dst, layer, len, acc, budget, recent, B, acc_out, len_out, kept]
+            const char* what = "kvEvictQ4";
+            Buf& kv = find_buf(ctx, c[1], kQ4, what);
+            Buf& dst = find_buf(ctx, c[2], kQ4, what);
+            Q4EvictArgs a = {};
+            a.B = c[8]; a.G = kv.H; a.hd = kv.hd; a.srcMax = kv.maxSeq; a.dstMax = dst.maxSeq; a.budget = c[6]; a.recent = c[7];
+            a.src = q4_layer(kv, a.B, c[3], what); a.dst = q4_layer(dst, a.B, c[3], what);
+            require(dst.H == kv.H && dst.hd == kv.hd, what, "the caches differ in heads or head size");
+            require(a.budget >= 1 && a.budget <= dst.maxSeq && a.recent >= 0 && a.recent <= a.budget, what, "bad budget or number of recent rows");
+            require(a.B <= 65535, what, "too many sequences");
+            require(c[10] != c[4], what, "the lengths go to another buffer than they come from");
+            require(c[9] != c[5] || a.srcMax == a.dstMax, what, "weights that stay in place need caches of one size");
+            a.len = f32(ctx, c[4], a.B, what);
+            a.acc = f32(ctx, c[5], sz(a.B, a.G) * a.srcMax, what); a.accOut = f32(ctx, c[9], sz(a.B, a.G) * a.dstMax, what);
+            a.lenOut = f32(ctx, c[10], a.B, what); a.kept = f32_opt(ctx, c[11], sz(a.B, a.G) * a.budget, what);
+            if (go) launch_q4_evict(a, s);
+            break;
+        }
+        case DEEPJ_OP_KV_STORE_Q4: {   // [op, src, k_off, v_off, ld, kv, layer, at, B, T]
+            const char* what = "kvStoreQ4";
+            Buf& kv = find_buf(ctx, c[5], kQ4, what);
+            Q4AttnArgs a = {};
+            const int T = c[9];
+            a.B = c[8]; a.G = kv.H; a.hd = kv.hd; a.maxSeq = kv.maxSeq;
+            a.cache = q4_layer(kv, a.B, c[6], what);
+            require(T >= 0 && (long long)a.B * T <= 0x7fffffff, what, "bad number of rows");
+            a.M = a.B * T; a.k_off = c[2]; a.v_off = c[3]; a.ld = c[4];
+            require(a.k_off >= 0 && a.v_off >= 0 && a.k_off % 4 == 0 && a.v_off % 4 == 0 && a.ld % 4 == 0, what, "offsets and stride must be multiples of 4 floats");
+            const long long width = (long long)std::max(a.k_off, a.v_off) + (long long)a.G * a.hd;
+            require(a.ld >= width, what, "row stride smaller than the row");
+            a.qkv = f32(ctx, c[1], a.M ? sz(a.M - 1, a.ld) + width : 0, what);
+            a.len = f32(ctx, c[7], a.B, what);
+            if (go && a.M) launch_q4_append(a, T, s);
+            break;
+        }
+        case DEEPJ_OP_KV_LOAD_Q4: {   // [op, kv, layer, at, end, T, k_out, v_out, B]
+            const char* what = "kvLoadQ4";
+            Buf& kv = find_buf(ctx, c[1], kQ4, what);
+            Q4LoadArgs a = {};
+            a.B = c[8]; a.G = kv.H; a.hd = kv.hd; a.maxSeq = kv.maxSeq; a.T = c[5];
+            a.cache = q4_layer(kv, a.B, c[2], what);
+            require(a.T >= 0 && sz(a.B, a.G) <= 65535, what, "bad number of rows or heads");
+            a.at = f32_opt(ctx, c[3], a.B, what); a.end = f32_opt(ctx, c[4], a.B, what);
+            a.k = f32(ctx, c[6], sz(a.B, a.G) * a.T * a.hd, what); a.v = f32(ctx, c[7], sz(a.B, a.G) * a.T * a.hd, what);
+            if (go) launch_q4_load(a, s);
             break;
         }
         case DEEPJ_OP_BF16_BLOCK_LINEAR: {   // [op, x, x_off, ldx, xstr, w, heads, out, out_off, ldo, ostr, M]
@@ -1292,6 +1389,33 @@ int deepj_cuda_kv_alloc(int32_t id, int32_t layers, int32_t batch, int32_t heads
 }
 int deepj_cuda_kv_alloc_f16(int32_t id, int32_t layers, int32_t batch, int32_t heads, int32_t max_seq, int32_t head_dim) {
     return kv_alloc_impl(id, layers, batch, heads, max_seq, head_dim, 1);
+}
+
+int deepj_cuda_kv_alloc_q4(int32_t id, int32_t layers, int32_t batch, int32_t kv_heads, int32_t max_seq, int32_t head_dim) {
+    DJ_TRY
+    ensure_init();
+    part(q4_plane_bytes, "kv_alloc_q4");
+    if (layers <= 0 || batch <= 0 || kv_heads <= 0 || max_seq <= 0) throw std::runtime_error("kv_alloc_q4: dimensions must be positive");
+    if (head_dim != 32 && head_dim != 64 && head_dim != 128) throw std::runtime_error("kv_alloc_q4: the head dim must be 32, 64 or 128");
+    if (max_seq > 1 << 24) throw std::runtime_error("kv_alloc_q4: lengths travel as floats, which count to 2^24");
+    if (R.pool.count(id)) throw std::runtime_error("kv_alloc_q4: id " + std::to_string(id) + " already exists");
+    Buf b; b.kind = kQ4; b.layers = layers; b.B = batch; b.H = kv_heads; b.maxSeq = max_seq; b.hd = head_dim;
+    b.bytes = (size_t)layers * q4_plane_bytes(batch, kv_heads, max_seq, head_dim);
+    DJ_CUDA_CHECK(device_malloc(&b.ptr, b.bytes));
+    DJ_CUDA_CHECK(cudaMemsetAsync(b.ptr, 0, b.bytes, R.stream));
+    b.serial = R.next_serial++;
+    R.pool[id] = b;
+    DJ_CATCH
+}
+
+int deepj_cuda_buffer_address(int32_t id, uint64_t* address, int64_t* floats) {
+    DJ_TRY
+    auto it = R.pool.find(id);
+    if (it == R.pool.end() || it->second.kind != kF32 || it->second.ptr == nullptr) throw std::runtime_error("buffer_address: id " + std::to_string(id) + " is no float buffer");
+    if (address == nullptr || floats == nullptr) throw std::runtime_error("buffer_address: null output");
+    *address = (uint64_t)(uintptr_t)it->second.ptr;
+    *floats = (int64_t)it->second.floats;
+    DJ_CATCH
 }
 
 }  // extern "C"

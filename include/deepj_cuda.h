@@ -123,6 +123,17 @@ int deepj_cuda_kv_alloc(int32_t kv_id, int32_t layers, int32_t batch, int32_t he
 int deepj_cuda_kv_alloc_f16(int32_t kv_id, int32_t layers, int32_t batch, int32_t heads,
                             int32_t max_seq, int32_t head_dim);
 
+/* The same kind of object in 4 bits, for ops 87 - 91: kv_heads key/value heads (any number of query heads may share one), head_dim 32, 64 or
+ * 128.  Every row is cut into blocks of 32 values: scale = bf16(max|w| * fp32(1/7)), at least 2^-17 and at most 2^13 (0 for a block of zeros), code =
+ * clamp(round-half-even(w / scale), -7, 7), NaN -> 0; a row reads back as code * scale.  Keys are rotated in fp32 before they are quantized.
+ * 1.125 * head_dim bytes hold a key and a value row.  How many rows a sequence has is the caller's (`len`, a float buffer), apart from the
+ * position its next token is rotated at (`pos`): after an eviction the two differ.  max_seq <= 2^24. */
+int deepj_cuda_kv_alloc_q4(int32_t kv_id, int32_t layers, int32_t batch, int32_t kv_heads, int32_t max_seq, int32_t head_dim);
+
+/* Device address and size of a float buffer, for other libraries on the device (no copy).  Work of other streams on it is the caller's to order:
+ * deepj_cuda_synchronize before they read what a flush wrote, their own wait before a flush reads what they wrote.  Ends with the buffer. */
+int deepj_cuda_buffer_address(int32_t id, uint64_t* address, int64_t* floats);
+
 /* Decode plan: everything one batch-1 token step of a Llama-shaped Q8 model touches, resolved once, for op 76
  * (DECODE_STEP), which runs the whole step — embedding row, every block, final norm, LM head, greedy pick, position
  * advance — as ONE persistent kernel.  No counterpart in the reference (its step is DecoderOnlyModel.forward over the
@@ -296,6 +307,27 @@ int deepj_cuda_latent_alloc(int32_t id, int32_t batch, int32_t max_seq, int32_t 
  *                        B, T, H, dim, vdim, exact]   matrix-memory recurrence with exponential gates over T tokens of B
  *                        sequences; state [B][H][vdim][dim] and norm [2][B][H][dim + 1] carried in fp32; a sequence at
  *                        position 0 starts from zeros (csrc/mlstm.cu)
+ *
+ * Ops over a 4-bit cache (deepj_cuda_kv_alloc_q4), H query heads over its G key/value heads, H a multiple of G.  A sequence whose length is
+ * outside 0 … max_seq - 1 or whose position is outside 0 … max_pos - 1 is left out: nothing of it is appended or written.  Tokens that
+ * do not fit (behind max_seq rows or max_pos positions) are left out as well.  Offsets and strides are multiples of four floats.
+ *
+ *  87 ATTN_DECODE_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, acc, acc_out]
+ *                        one token of every sequence: q and k rotated at pos[b] (tables [max_pos][hd/2]), k and v appended as row len[b], softmax
+ *                        attention over rows 0..len[b].  acc, acc_out [B][G][max_seq] (or both -1; may be one buffer): acc_out of row j =
+ *                        (j < len[b] ? acc : 0) + the softmax weights that the G's query heads give row j; entries beyond len[b] stay
+ *  88 ATTN_PACKED_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, starts, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, M, acc, acc_out, window]
+ *                        prompts of different lengths: rows starts[b] .. starts[b+1]-1 of the M rows are the tokens of sequence b (none is fine; rows
+ *                        of no sequence stay as they are; ranges must not overlap).  Token t is rotated at pos[b] + t, appended as row len[b] + t and
+ *                        attends to rows 0..len[b]+t.  acc / acc_out as above with the weights of the sequence's last `window` tokens (>= 1);
+ *                        window = 0 with acc = acc_out = -1
+ *  89 KV_EVICT_Q4       [op, kv, dst, layer, len, acc, budget, recent, B, acc_out, len_out, kept]
+ *                        of len[b] > budget rows keeps the newest `recent` and the budget - recent others with the largest acc (equal ones: the
+ *                        earlier row; NaN: last), in order, in `dst` (the same object, or one of the same heads and layers); acc_out [B][G][max_seq of dst]
+ *                        (may be acc), len_out[b] = rows kept (another buffer than len), kept [B][G][budget] their former rows, or -1
+ *  90 KV_STORE_Q4       [op, src, k_off, v_off, ld, kv, layer, at, B, T]      row b*T + t of src becomes row at[b] + t of sequence b, as it is
+ *  91 KV_LOAD_Q4        [op, kv, layer, at, end, T, k_out, v_out, B]          values of rows at[b] + t < end[b], t < T, as [B][G][T][hd]; at = -1: from
+ *                        row 0, end = -1: to max_seq; other rows of the outputs stay as they are
  */
 #define DEEPJ_OP_EMBED_GATHER        64
 #define DEEPJ_OP_Q8_LINEAR           65
@@ -320,6 +352,11 @@ int deepj_cuda_latent_alloc(int32_t id, int32_t batch, int32_t max_seq, int32_t 
 #define DEEPJ_OP_NORM_ADD           84
 #define DEEPJ_OP_ATTN_GROUPED       85
 #define DEEPJ_OP_MLSTM              86
+#define DEEPJ_OP_ATTN_DECODE_Q4     87
+#define DEEPJ_OP_ATTN_PACKED_Q4     88
+#define DEEPJ_OP_KV_EVICT_Q4        89
+#define DEEPJ_OP_KV_STORE_Q4        90
+#define DEEPJ_OP_KV_LOAD_Q4         91
 
 #ifdef __cplusplus
 }
