@@ -126,7 +126,7 @@ DJ_PART int attn_decode_splits(int B, int H, int maxSeq);
 DJ_PART void launch_attn_decode(const AttnDecodeArgs& a, cudaStream_t s);
 DJ_PART bool launch_attn_prefill_mma(const AttnDecodeArgs& a, cudaStream_t s);     // prompt chunks on the tensor cores (head dim 64 / 128)
 
-// ── attention over a 4-bit cache (q4_cache.cu, q4_attn.cu) ──
+// ── attention over a 4-bit cache (q4_cache.cu, q4_decode.cu, q4_attn.cu) ──
 struct Q4AttnArgs {
     const float* qkv; int q_off, k_off, v_off, ld;       // one row per token: H query heads, G key and G value heads of hd values
     unsigned char* cache; int maxSeq;                    // this layer's pages [B][G][ceil(maxSeq / 32)] (q4_cache.cuh)
@@ -136,7 +136,8 @@ struct Q4AttnArgs {
     float* out; int ldo;                                 // [M × H·hd]
     int B, H, G, hd, M;
     const float* acc; float* accOut; int window;         // [B][G][maxSeq] accumulated weights, of the last `window` tokens; null: none
-    float* ws; int* tickets;
+    int early;                                           // the cache may be read before the dependency wait
+    float* ws;
 };
 struct Q4LoadArgs { const unsigned char* cache; int maxSeq; const float* at; const float* end; float* k; float* v; int B, G, hd, T; };
 struct Q4EvictArgs {
@@ -147,6 +148,8 @@ DJ_PART size_t q4_plane_bytes(int B, int G, int maxSeq, int hd);
 DJ_PART size_t q4_attn_ws_floats(const Q4AttnArgs& a);
 DJ_PART void launch_q4_append(const Q4AttnArgs& a, int T, cudaStream_t s);      // rows only; T tokens per sequence where starts is null
 DJ_PART void launch_q4_attn(const Q4AttnArgs& a, cudaStream_t s);               // append and attend
+DJ_PART size_t q4_decode_ws_floats(const Q4AttnArgs& a);
+DJ_PART void launch_q4_decode(const Q4AttnArgs& a, cudaStream_t s);             // the same for one token of every sequence (q4_decode.cu)
 DJ_PART void launch_q4_load(const Q4LoadArgs& a, cudaStream_t s);
 DJ_PART void launch_q4_evict(const Q4EvictArgs& a, cudaStream_t s);
 

@@ -30,7 +30,7 @@ template <int NB>
 __device__ __forceinline__ float dim_of(const unsigned char* page, int r, int j, int lane, bool value) {
     const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(r, lane >> 2 & 3, j));
     const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (r * NB + j) * 2));
-    return (float)((int)(w >> (8 * (lane & 3) + (lane >> 4) * 4) & 15) - 8) * s;          // dim 32j + lane
+    return (float)q4_code(w, 8 * (lane & 3) + (lane >> 4) * 4) * s;          // dim 32j + lane
 }
 
 template <int NB>

@@ -90,9 +90,9 @@ __global__ void __launch_bounds__(256) k_q4_load(const LoadParams p) {
         const size_t to = ((size_t)bg * p.T + i) * (32 * NB) + 4 * e;
 #pragma unroll
         for (int value = 0; value < 2; value++) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(r, t, j)) >> shift;
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(r, t, j));
             const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (r * NB + j) * 2));
-            auto val = [&](int k) { return (float)((int)(w >> (8 * k) & 15) - 8) * s; };
+            auto val = [&](int k) { return (float)q4_code(w, 8 * k + shift) * s; };
             *reinterpret_cast<float4*>((value ? p.v : p.k) + to) = make_float4(val(0), val(1), val(2), val(3));
         }
     }

@@ -6,8 +6,8 @@
 // range of s, which is what lets the tensor cores multiply stored values without a correction term.
 // Rows lie in pages of 32 consecutive positions, 1152·NB contiguous bytes that one bulk copy brings:
 //     K codes [32][16·NB] | V codes [32][16·NB] | K scales [32][NB] bf16 | V scales [32][NB] bf16
-// Word (t, j) of a row, t < 4, j < NB, holds as nibbles code + 8: byte i the dims 32j + 4t + i (low) and 32j + 16 + 4t + i (high), so that masking
-// a word gives two operand registers of m16n8k32.  The words of one t are a piece of 4·NB bytes; piece t of row r sits in slot t ^ (r/2 % 4): with
+// Word (t, j) of a row, t < 4, j < NB, holds the codes as two's complement nibbles: byte i the dims 32j + 4t + i (low) and 32j + 16 + 4t + i (high).
+// Masked, a word gives two int8 operand registers of m16n8k32 whose bytes are 16 times the codes.  The words of one t are a piece of 4·NB bytes; piece t of row r sits in slot t ^ (r/2 % 4): with
 // rows of 64 bytes the warp that reads one piece of four consecutive rows finds them in different banks.
 #pragma once
 #include <cuda_bf16.h>
@@ -32,7 +32,7 @@ __device__ __forceinline__ int q4_room(int tokens, int len, int maxSeq, int pos,
     return max(0, min(tokens, min(maxSeq - len, maxPos - pos)));
 }
 
-// The eight lanes of a block hold four values each → the block's scale and this lane's four codes + 8 in the low nibbles of a word's bytes.
+// The eight lanes of a block hold four values each → the block's scale and this lane's four codes in the low nibbles of a word's bytes.
 __device__ __forceinline__ uint32_t q4_codes(float4 x, float& scale) {
     x.x = x.x == x.x ? x.x : 0.0f; x.y = x.y == x.y ? x.y : 0.0f; x.z = x.z == x.z ? x.z : 0.0f; x.w = x.w == x.w ? x.w : 0.0f;
     float most = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t q4_codes(float4 x, float& scale) {
     for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     const float s = fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(most * (1.0f / 7.0f))), kQ4ScaleMin), kQ4ScaleMax);
     scale = most > 0.0f ? s : 0.0f;
-    auto code = [&](float v) { return (uint32_t)((int)fminf(fmaxf(rintf(v / s), -7.0f), 7.0f) + 8); };
+    auto code = [&](float v) { return (uint32_t)((int)fminf(fmaxf(rintf(v / s), -7.0f), 7.0f)) & 15u; };
     return code(x.x) | code(x.y) << 8 | code(x.z) << 16 | code(x.w) << 24;
 }
 
@@ -59,5 +59,11 @@ __device__ __forceinline__ void q4_put_row(unsigned char* page, int row, bool va
 __device__ __forceinline__ float4 q4_rotate(const float4& x, const float2& c, const float2& s) {
     return make_float4(x.x * c.x - x.y * s.x, x.x * s.x + x.y * c.x, x.z * c.y - x.w * s.y, x.z * s.y + x.w * c.y);
 }
+
+// A word's codes in the high (low: shifted there) nibbles of its bytes: int8 values of 16 times the code.
+__device__ __forceinline__ uint32_t q4_high(uint32_t w) { return w & 0xf0f0f0f0u; }
+__device__ __forceinline__ uint32_t q4_low(uint32_t w) { return (w << 4) & 0xf0f0f0f0u; }
+// one code of a word: bit 0 of its nibble is at `shift`
+__device__ __forceinline__ int q4_code(uint32_t w, int shift) { return (int)(w << (28 - shift)) >> 28; }
 
 }  // namespace dj

@@ -194,6 +194,7 @@ struct Ctx {
     size_t ws_need = 0;
     int prev_op = 0;                   // op code before this one in the stream
     const int32_t* prev = nullptr;     // and its words
+    const int32_t* solid = nullptr;    // words of the last op before this one that is no Q8 projection
     int next_op = 0;                   // op code behind this one, 0 = none
     bool bounded_waits = false;        // the stream holds an op whose kernel waits on a peer (tensor-parallel exchange)
     std::vector<std::pair<int, unsigned long long>>* refs = nullptr;
@@ -336,6 +337,11 @@ void do_op(Ctx& ctx, const int32_t* c) {
     // A projection lets the kernel behind it in before its own wait where that one reads nothing but weights ahead of its wait
     // (every older kernel may still run then, so nothing that keeps a state or a cache).
     const bool trigger = ctx.next_op == DEEPJ_OP_BF16_LINEAR || ctx.next_op == DEEPJ_OP_BF16_LINEAR_SUM || ctx.next_op == DEEPJ_OP_NORM_ADD;
+    // Q8 projections let the kernel behind them in before their own wait.  Behind any other op of this stream everything older is complete, so a cache
+    // may be read ahead of the wait behind projections that follow one which does not write that cache.
+    const bool q8 = op == DEEPJ_OP_Q8_LINEAR || op == DEEPJ_OP_Q8_LINEAR_LN || op == DEEPJ_OP_Q8_SWIGLU;
+    const int32_t* const solid = ctx.solid;
+    if (!q8) ctx.solid = c;
     const int32_t* const prev = ctx.prev;
     ctx.prev_op = op; ctx.prev = c;
     auto scratch = [&](size_t floats) {          // room in the shared workspace for this op
@@ -760,9 +766,10 @@ void do_op(Ctx& ctx, const int32_t* c) {
             require((w[0] < 0) == (w[1] < 0), what, "accumulated weights need both an input and an output (which may be the same buffer)");
             require(!packed || (w[0] < 0) == (a.window == 0), what, "a window goes with accumulated weights, and they with a window");
             a.acc = f32_opt(ctx, w[0], sz(a.B, a.G) * a.maxSeq, what); a.accOut = f32_opt(ctx, w[1], sz(a.B, a.G) * a.maxSeq, what);
-            a.tickets = R.tickets;
-            a.ws = scratch(q4_attn_ws_floats(a));
-            if (go) launch_q4_attn(a, s);
+            a.early = solid != nullptr && solid != prev && solid[0] != DEEPJ_OP_ATTN_PACKED_Q4 && solid[0] != DEEPJ_OP_KV_EVICT_Q4 && solid[0] != DEEPJ_OP_KV_STORE_Q4 &&
+                      !(solid[0] == DEEPJ_OP_ATTN_DECODE_Q4 && solid[6] == c[6] && solid[7] == c[7]);
+            a.ws = scratch(packed ? q4_attn_ws_floats(a) : q4_decode_ws_floats(a));
+            if (go) { if (packed) launch_q4_attn(a, s); else launch_q4_decode(a, s); }
             break;
         }
         case DEEPJ_OP_KV_EVICT_Q4: {   // [op, kv, dst, layer, len, acc, budget, recent, B, acc_out, len_out, kept]
