@@ -126,7 +126,7 @@ DJ_PART int attn_decode_splits(int B, int H, int maxSeq);
 DJ_PART void launch_attn_decode(const AttnDecodeArgs& a, cudaStream_t s);
 DJ_PART bool launch_attn_prefill_mma(const AttnDecodeArgs& a, cudaStream_t s);     // prompt chunks on the tensor cores (head dim 64 / 128)
 
-// ── attention over a 4-bit cache (q4_cache.cu, q4_decode.cu, q4_attn.cu) ──
+// ── attention over a 4-bit cache (q4_cache.cu, q4_decode.cu, q4_prefill.cu) ──
 struct Q4AttnArgs {
     const float* qkv; int q_off, k_off, v_off, ld;       // one row per token: H query heads, G key and G value heads of hd values
     unsigned char* cache; int maxSeq;                    // this layer's pages [B][G][ceil(maxSeq / 32)] (q4_cache.cuh)

@@ -5,7 +5,7 @@
 // and 32 codes clamp(round_half_even(w / s), -7, 7), NaN → 0.  A code has 3 bits and a sign, s has 8 bits: code · s is exact in fp16 over the whole
 // range of s, which is what lets the tensor cores multiply stored values without a correction term.
 // Rows lie in pages of 32 consecutive positions, 1152·NB contiguous bytes that one bulk copy brings:
-//     K codes [32][16·NB] | V codes [32][16·NB] | K scales [32][NB] bf16 | V scales [32][NB] bf16
+//     K codes [32][16·NB] | K scales [32][NB] bf16 | V codes [32][16·NB] | V scales [32][NB] bf16
 // Word (t, j) of a row, t < 4, j < NB, holds the codes as two's complement nibbles: byte i the dims 32j + 4t + i (low) and 32j + 16 + 4t + i (high).
 // Masked, a word gives two int8 operand registers of m16n8k32 whose bytes are 16 times the codes.  The words of one t are a piece of 4·NB bytes; piece t of row r sits in slot t ^ (r/2 % 4): with
 // rows of 64 bytes the warp that reads one piece of four consecutive rows finds them in different banks.
@@ -21,8 +21,8 @@ constexpr int kQ4PageBytes = 1152;               // … times NB
 constexpr float kQ4ScaleMin = 1.0f / 131072.0f, kQ4ScaleMax = 8192.0f;
 
 template <int NB> struct Q4Page {
-    static constexpr int kBytes = kQ4PageBytes * NB, kRow = 16 * NB;
-    static constexpr int kV = kQ4Page * kRow, kKs = 2 * kV, kVs = kKs + kQ4Page * NB * 2;      // offsets of the V codes and of the scales
+    static constexpr int kBytes = kQ4PageBytes * NB, kHalf = kBytes / 2, kRow = 16 * NB;
+    static constexpr int kKs = kQ4Page * kRow, kV = kHalf, kVs = kV + kKs;                     // offsets of the scales and of the V half
     static __device__ __forceinline__ int word(int row, int t, int j) { return row * kRow + (t ^ ((row >> 1) & 3)) * (4 * NB) + 4 * j; }
 };
 

@@ -749,7 +749,7 @@ void do_op(Ctx& ctx, const int32_t* c) {
             a.M = packed ? c[19] : a.B; a.window = packed ? c[22] : 1;
             require(a.M >= 0 && a.window >= 0 && a.maxPos >= 1, what, "bad dimension");
             require(a.H >= 1 && a.H % a.G == 0 && a.H / a.G <= 64, what, "query heads must be a multiple (at most 64 times) of the cache's heads");
-            require((long long)a.H * a.hd <= 1 << 20 && a.G <= 65535, what, "too many heads");
+            require((long long)a.H * a.hd <= 1 << 20 && (long long)a.G * ((a.H / a.G + 3) / 4) <= 65535 && a.B <= 65535, what, "too many heads or sequences");
             a.q_off = c[2]; a.k_off = c[3]; a.v_off = c[4]; a.ld = c[5];
             require(a.q_off >= 0 && a.k_off >= 0 && a.v_off >= 0 && e[14] >= 0, what, "negative offset");
             require(a.ld % 4 == 0 && a.q_off % 4 == 0 && a.k_off % 4 == 0 && a.v_off % 4 == 0 && e[14] % 4 == 0 && e[15] % 4 == 0, what,
