@@ -28,7 +28,8 @@ import numpy as np
 
 from . import _lib
 from .runner import StreamDecoder
-from .compute_graph import (OP_ADD, OP_DECODE_STEP, OP_Q8_LINEAR_LN, OP_ADD_SCALAR_INPLACE, OP_ARGMAX_ROWS, OP_ATTN_DECODE, OP_ATTN_PREFILL, OP_COPY, OP_EMBED_GATHER, OP_SAMPLE_TOPK,
+from .compute_graph import (OP_ADD, OP_DECODE_STEP, OP_Q8_LINEAR_LN, OP_ADD_SCALAR_INPLACE, OP_ARGMAX_ROWS, OP_ATTN_DECODE, OP_ATTN_DECODE_Q4, OP_ATTN_PACKED_Q4,
+                            OP_ATTN_PREFILL, OP_COPY, OP_EMBED_GATHER, OP_KV_EVICT_Q4, OP_SAMPLE_TOPK,
                             OP_Q8_LINEAR, OP_Q8_SWIGLU, OP_TP_ALLGATHER, OP_TP_ALLREDUCE, float_bits)
 
 RMS_EPS = 1e-6      # layers/transformer/norm/RMSNorm1D.java:30
@@ -89,8 +90,8 @@ class DecoderConfig:
         return per_layer * self.n_layers + q8(self.d_model, self.vocab_size)
 
     def kv_bytes_per_position(self, kv_dtype: str = "f32") -> int:
-        """K and V rows of one cached position, all layers (fp32, or fp16 with kv_dtype "f16")."""
-        return 2 * self.n_layers * self.d_model * (2 if kv_dtype == "f16" else 4)
+        """K and V rows of one cached position, all layers (fp32, fp16 with kv_dtype "f16", 4-bit codes and their scales with "q4")."""
+        return 2 * self.n_layers * self.d_model * {"f32": 64, "f16": 32, "q4": 9}[kv_dtype] // 16
 
 
 def rope_tables(head_dim: int, max_seq: int):
@@ -158,7 +159,8 @@ class Q8Decoder(StreamDecoder):
 
     def __init__(self, cfg: DecoderConfig, batch: int = 1, device: int = 0, id_base: int = 1 << 24,
                  tp_rank: int = 0, tp_world: int = 1, tp_slot_floats: int = 0, share_weights: Optional["Q8Decoder"] = None,
-                 fused_step: Optional[bool] = None, kv_dtype: str = "f32"):
+                 fused_step: Optional[bool] = None, kv_dtype: str = "f32", kv_rows: Optional[int] = None, kv_budget: Optional[int] = None,
+                 kv_recent: Optional[int] = None):
         """`tp_slot_floats`: the slot size the exchange buffer was (or will be) connected with (`tp.connect`); it
         bounds the rows a tensor-parallel prompt chunk may have (rows × dModel floats per exchange).
         `share_weights`: another decoder of the same configuration and sharding whose device weights this one reads
@@ -167,9 +169,27 @@ class Q8Decoder(StreamDecoder):
         qualify (a Llama-shaped model, one sequence, every reduction length a multiple of 32, head dim 32 / 64 / 128).
         Under tensor parallelism the plan is made at the first step, after `tp.connect`.
         `kv_dtype`: "f32" (the reference's precision) or "f16" — keys rounded after the rotation, values rounded, fp32
-        arithmetic; half the bytes a step's attention reads."""
-        if kv_dtype not in ("f32", "f16"):
-            raise ValueError("kv_dtype must be 'f32' or 'f16'")
+        arithmetic; half the bytes a step's attention reads — or "q4": 4-bit codes with a scale to 32 values, a seventh of the fp32 bytes,
+        prompts of different lengths (`prefill_packed`).  `kv_rows` ("q4"): cached rows per sequence, at most `max_seq_len`, which is the
+        default.  `kv_budget`: a cache without room for the next tokens is cut to so many rows, the newest `kv_recent` (default: a quarter
+        of them) and those that got the most attention so far; without a budget a full cache is an error."""
+        if kv_dtype not in ("f32", "f16", "q4"):
+            raise ValueError("kv_dtype must be 'f32', 'f16' or 'q4'")
+        if kv_dtype != "q4" and (kv_rows, kv_budget, kv_recent) != (None, None, None):
+            raise ValueError("kv_rows, kv_budget and kv_recent go with a 4-bit cache")
+        if kv_dtype == "q4":
+            if fused_step or cfg.head_dim not in (32, 64, 128):
+                raise ValueError("a 4-bit KV cache needs a head dim of 32, 64 or 128 and the per-operator step")
+            self.kv_rows = cfg.max_seq_len if kv_rows is None else int(kv_rows)
+            if not 1 <= self.kv_rows <= cfg.max_seq_len:
+                raise ValueError("kv_rows must be in 1..maxSeqLen")
+            if kv_budget is None and kv_recent is not None:
+                raise ValueError("kv_recent goes with a budget")
+            self.kv_budget = None if kv_budget is None else int(kv_budget)
+            if self.kv_budget is not None:
+                self.kv_recent = self.kv_budget // 4 if kv_recent is None else int(kv_recent)
+                if not 1 <= self.kv_budget < self.kv_rows or not 0 <= self.kv_recent <= self.kv_budget:
+                    raise ValueError("kv_budget must be in 1..kv_rows - 1 and kv_recent in 0..kv_budget")
         if kv_dtype == "f16" and (fused_step or cfg.head_dim % 16 != 0):
             raise ValueError("an fp16 KV cache needs a head dim that is a multiple of 16 and the per-operator step")
         self.kv_dtype = kv_dtype
@@ -240,8 +260,17 @@ class Q8Decoder(StreamDecoder):
         if c.kind == "deepseek":
             self._f32("lat", B * (c.q_rank + c.kv_rank))
         kv = self._new_id()
-        alloc = self.lib.deepj_cuda_kv_alloc_f16 if self.kv_dtype == "f16" else self.lib.deepj_cuda_kv_alloc
-        _lib.check(alloc(kv, c.n_layers, B, self.h_local, c.max_seq_len, c.head_dim))
+        if self.kv_dtype == "q4":
+            _lib.check(self.lib.deepj_cuda_kv_alloc_q4(kv, c.n_layers, B, self.h_local, self.kv_rows, c.head_dim))
+            self._rows = np.zeros(B, dtype=np.int64)         # cached rows of every sequence: "len" on the device
+            self._f32("len", B)
+            if self.kv_budget is not None:
+                self._f32("len_kept", B)
+                for l in range(c.n_layers):
+                    self._f32(f"seen.{l}", B * self.h_local * self.kv_rows)      # attention every cached row has got so far
+        else:
+            alloc = self.lib.deepj_cuda_kv_alloc_f16 if self.kv_dtype == "f16" else self.lib.deepj_cuda_kv_alloc
+            _lib.check(alloc(kv, c.n_layers, B, self.h_local, c.max_seq_len, c.head_dim))
         self.ids["kv"] = kv
 
     # ── weights ──
@@ -354,7 +383,7 @@ class Q8Decoder(StreamDecoder):
     def _build(self, feed_back: bool, sampler: Optional[Tuple[int, float]] = None) -> np.ndarray:
         c, B, I = self.cfg, self.B, self.ids
         d, V = c.d_model, c.vocab_size
-        dl, Fl, Vl, Hl = self.d_local, self.f_local, self.v_local, self.h_local
+        dl, Fl, Vl = self.d_local, self.f_local, self.v_local
         tp = self.tp_world > 1
         eps = float_bits(RMS_EPS)
         s: List[int] = []
@@ -383,8 +412,7 @@ class Q8Decoder(StreamDecoder):
                 linear("mla_down", I["x"], 0, d, I[f"g1.{l}"], I[f"Wdqkv.{l}"], -1, -1, 0, 0, I["lat"], 0, r)
                 linear("mla_up_q", I["lat"], 0, r, -1, I[f"Wuq.{l}"], -1, -1, 0, 0, I["qkv"], 0, 3 * dl)
                 linear("mla_up_kv", I["lat"], c.q_rank, r, -1, I[f"Wukv.{l}"], -1, -1, 0, 0, I["qkv"], dl, 3 * dl)
-            op("attn", OP_ATTN_DECODE, I["qkv"], 0, dl, 2 * dl, 3 * dl, I["kv"], l, I["pos"], I["cos"], I["sin"],
-               I["att"], 0, dl, B, Hl, c.head_dim)
+            op("attn", *self._attention(l, I["qkv"], I["att"], B, 1))
             if tp:
                 # row-parallel: every rank holds a partial sum; the exchange adds them (+ residual, + bias)
                 linear("wo", I["att"], 0, dl, -1, I[f"Wo.{l}"], -1, -1, 0, 0, I["part"], 0, d)
@@ -408,28 +436,41 @@ class Q8Decoder(StreamDecoder):
         else:
             op("sample", OP_SAMPLE_TOPK, I["logits"], I["r"], I["next"], B, V, sampler[0], float_bits(sampler[1]))
         op("advance", OP_ADD_SCALAR_INPLACE, I["pos"], float_bits(1.0), B)
+        if self.kv_dtype == "q4":
+            op("advance_rows", OP_ADD_SCALAR_INPLACE, I["len"], float_bits(1.0), B)
         if feed_back:
             op("feed_back", OP_COPY, I["next"], 0, I["tok"], 0, B)
         self._op_labels = labels
         self._op_bounds = bounds
         return np.asarray(s, dtype=np.int32)
 
-    def _gpt_blocks(self, op, x, x2, xp, qkv, att, h, pos_ids, B: int, T: int) -> None:
-        """The GPT part of a stream between the token gather and the final norm, for M = B·T rows: add the learned
+    WINDOW = 32              # prompt tokens at the end of a chunk whose attention counts towards what stays in a bounded cache
+
+    def _attention(self, l: int, qkv: int, att: int, rows: int, T: int, chunk: bool = False) -> List[int]:
+        """The attention op of layer l: T tokens of every sequence (one: a step, unless it is a chunk's), or `rows` packed ones (T = 0)."""
+        c, B, I, dl = self.cfg, self.B, self.ids, self.d_local
+        fields = [qkv, 0, dl, 2 * dl, 3 * dl, I["kv"], l]
+        if self.kv_dtype != "q4":
+            tail = [I["pos"], I["cos"], I["sin"], att, 0, dl, B, self.h_local, c.head_dim]
+            return [OP_ATTN_PREFILL] + fields + tail + [T] if chunk or T != 1 else [OP_ATTN_DECODE] + fields + tail
+        seen = -1 if self.kv_budget is None else I[f"seen.{l}"]
+        where = [I["len"], I["pos"], I["cos"], I["sin"], c.max_seq_len, att, 0, dl, B, self.h_local]
+        if T == 1:
+            return [OP_ATTN_DECODE_Q4] + fields + where + [seen, seen]
+        return [OP_ATTN_PACKED_Q4] + fields + [self._prefill_ids["starts"]] + where + [rows, seen, seen, 0 if seen < 0 else self.WINDOW]
+
+    def _gpt_blocks(self, op, x, x2, xp, qkv, att, h, pos_ids, M: int, T: int) -> None:
+        """The GPT part of a stream between the token gather and the final norm, for M rows (T of every sequence; T = 0: packed): add the learned
         position rows (embeddings/PositionalEmbedding.java:26-33; `pos_ids` holds one position per row), then per
         block LayerNorm→QKV, attention, Wo + residual, LayerNorm→W1 + c1→GELU, W2 + c2 + residual."""
         c, I = self.cfg, self.ids
-        d, F, M = c.d_model, c.d_ff, B * T
+        d, F = c.d_model, c.d_ff
         eps = float_bits(LN_EPS)
         op("pos_embed", OP_EMBED_GATHER, I["posemb"], pos_ids, xp, M, d, c.max_seq_len)
         op("pos_add", OP_ADD, x, xp, x, M * d)
         for l in range(c.n_layers):
             op("qkv", OP_Q8_LINEAR_LN, x, 0, d, I[f"g1.{l}"], I[f"b1.{l}"], eps, I[f"Wqkv.{l}"], -1, -1, 0, 0, qkv, 0, 3 * d, M, 0)
-            if T == 1:
-                op("attn", OP_ATTN_DECODE, qkv, 0, d, 2 * d, 3 * d, I["kv"], l, I["pos"], I["cos"], I["sin"], att, 0, d, B, c.n_heads, c.head_dim)
-            else:
-                op("attn", OP_ATTN_PREFILL, qkv, 0, d, 2 * d, 3 * d, I["kv"], l, I["pos"], I["cos"], I["sin"], att, 0, d, B, c.n_heads,
-                   c.head_dim, T)
+            op("attn", *self._attention(l, qkv, att, M, T))
             op("wo", OP_Q8_LINEAR, att, 0, d, -1, 0, I[f"Wo.{l}"], -1, x, 0, d, x2, 0, d, M)
             op("ffn_up", OP_Q8_LINEAR_LN, x2, 0, d, I[f"g2.{l}"], I[f"b2.{l}"], eps, I[f"W1.{l}"], I[f"c1.{l}"], -1, 0, 0, h, 0, F, M, 1)
             op("ffn_down", OP_Q8_LINEAR, h, 0, F, -1, 0, I[f"W2.{l}"], I[f"c2.{l}"], x2, 0, d, x, 0, d, M)
@@ -469,14 +510,15 @@ class Q8Decoder(StreamDecoder):
             _lib.check(self.lib.deepj_cuda_flush_ops(g.ctypes.data, g.size))
         return super().logits()
 
-    def _build_prefill(self, T: int) -> np.ndarray:
+    def _build_prefill(self, T: int, ends: Optional[List[Tuple[int, int]]] = None, rows: int = 0) -> np.ndarray:
         """The stream of one prompt chunk: T tokens of every sequence at once, B·T activation rows through the
         many-row Q8 kernels and the chunk attention op; the last token's hidden state lands in the decode
         buffers and the positions advance by T.  The row-major layout is row = b·T + t.  Under tensor parallelism
-        the Wo and down projections leave partial sums that the exchange op adds over the ranks, M rows at a time."""
+        the Wo and down projections leave partial sums that the exchange op adds over the ranks, M rows at a time.
+        `ends` (with T = 0): `rows` packed rows instead, and (sequence, last row) of the sequences whose prompt ends here."""
         c, B, I, P = self.cfg, self.B, self.ids, self._prefill_ids
-        d, dl, Fl, Hl = c.d_model, self.d_local, self.f_local, self.h_local
-        M = B * T
+        d, dl, Fl = c.d_model, self.d_local, self.f_local
+        M = B * T if ends is None else rows
         eps = float_bits(RMS_EPS)
         s: List[int] = []
 
@@ -486,7 +528,7 @@ class Q8Decoder(StreamDecoder):
         s.extend((OP_EMBED_GATHER, I["emb"], P["tok"], P["x"], M, d, c.vocab_size))
         if c.kind == "gpt":
             self._gpt_blocks(lambda _label, *ints: s.extend(int(v) for v in ints), P["x"], P["x2"], P["xp"], P["qkv"], P["att"], P["h"],
-                             P["ppos"], B, T)
+                             P["ppos"], M, T)
         for l in range(c.n_layers if c.kind != "gpt" else 0):
             if c.kind == "llama":
                 linear(P["x"], 0, d, I[f"g1.{l}"], I[f"Wqkv.{l}"], -1, -1, 0, P["qkv"], 3 * dl)
@@ -495,8 +537,7 @@ class Q8Decoder(StreamDecoder):
                 linear(P["x"], 0, d, I[f"g1.{l}"], I[f"Wdqkv.{l}"], -1, -1, 0, P["lat"], r)
                 linear(P["lat"], 0, r, -1, I[f"Wuq.{l}"], -1, -1, 0, P["qkv"], 3 * dl)
                 s.extend(int(v) for v in (OP_Q8_LINEAR, P["lat"], c.q_rank, r, -1, eps, I[f"Wukv.{l}"], -1, -1, 0, 0, P["qkv"], dl, 3 * dl, M))
-            s.extend(int(v) for v in (OP_ATTN_PREFILL, P["qkv"], 0, dl, 2 * dl, 3 * dl, I["kv"], l, I["pos"], I["cos"], I["sin"],
-                                      P["att"], 0, dl, B, Hl, c.head_dim, T))
+            s.extend(self._attention(l, P["qkv"], P["att"], M, T, chunk=True))
             if self.tp_world > 1:       # row-parallel projections leave partial sums; the exchange adds them (+ residual, + bias)
                 linear(P["att"], 0, dl, -1, I[f"Wo.{l}"], -1, -1, 0, P["part"], d)
                 s.extend((OP_TP_ALLREDUCE, P["part"], -1, P["x"], P["x2"], M, d))
@@ -509,9 +550,12 @@ class Q8Decoder(StreamDecoder):
                 s.extend((OP_TP_ALLREDUCE, P["part"], I[f"bd.{l}"], P["x2"], P["x"], M, d))
             else:
                 linear(P["h"], 0, Fl, -1, I[f"Wd.{l}"], I[f"bd.{l}"], P["x2"], d, P["x"], d)
-        for b in range(B):
-            s.extend((OP_COPY, P["x"], (b * T + T - 1) * d, I["x"], b * d, d))
-        s.extend((OP_ADD_SCALAR_INPLACE, I["pos"], float_bits(float(T)), B))
+        for b, row in [(b, b * T + T - 1) for b in range(B)] if ends is None else ends:
+            s.extend((OP_COPY, P["x"], row * d, I["x"], b * d, d))
+        if ends is None:
+            s.extend((OP_ADD_SCALAR_INPLACE, I["pos"], float_bits(float(T)), B))
+            if self.kv_dtype == "q4":
+                s.extend((OP_ADD_SCALAR_INPLACE, I["len"], float_bits(float(T)), B))
         return np.asarray(s, dtype=np.int32)
 
     def _head_ops(self, x: int, logits: int, rows: int) -> List[int]:
@@ -532,6 +576,8 @@ class Q8Decoder(StreamDecoder):
 
     def _chunk_tokens(self) -> int:
         limit = super()._chunk_tokens()
+        if self.kv_dtype == "q4" and self.kv_budget is not None:
+            limit = min(limit, self.kv_rows - self.kv_budget)      # what fits behind an eviction
         return min(limit, self._tp_rows()) if self.tp_world > 1 else limit
 
     def prefill(self, prompts, chunked: Optional[bool] = None) -> np.ndarray:
@@ -547,8 +593,12 @@ class Q8Decoder(StreamDecoder):
 
     def _upload_chunk(self, tokens: np.ndarray) -> None:
         super()._upload_chunk(tokens)
+        if self.kv_dtype == "q4":
+            self._upload(self._prefill_ids["starts"], np.arange(self.B + 1, dtype=np.float32) * tokens.shape[1])
         if self.cfg.kind == "gpt":       # row b·T + t sits at position (start of the chunk) + t
             rows = np.tile(np.arange(self.position, self.position + tokens.shape[1], dtype=np.float32), self.B)
+            if self.kv_dtype == "q4":        # behind packed prompts every sequence has a position of its own
+                rows = (self._download(self.ids["pos"], self.B)[:, None] + np.arange(tokens.shape[1], dtype=np.float32)).reshape(-1)
             self._upload(self._prefill_ids["ppos"], rows)
 
     def _prefill_sizes(self, M: int) -> Dict[str, int]:
@@ -561,4 +611,97 @@ class Q8Decoder(StreamDecoder):
             sizes["xp"], sizes["ppos"] = M * c.d_model, M
         if self.tp_world > 1:
             sizes["part"] = M * c.d_model
+        if self.kv_dtype == "q4":
+            sizes["starts"] = self.B + 1
         return sizes
+
+    # ── the 4-bit cache ──
+    def _check_tokens(self, p: np.ndarray) -> None:
+        super()._check_tokens(p)
+        if self.kv_dtype == "q4" and self.kv_budget is None and int(self._rows.max()) + p.shape[1] > self.kv_rows:
+            raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+
+    def reset(self) -> None:
+        super().reset()
+        if self.kv_dtype == "q4":
+            self._set_rows(np.zeros(self.B, dtype=np.int64))
+
+    def set_position(self, position: int) -> None:
+        if self.kv_dtype == "q4" and position > self.kv_rows:
+            raise ValueError(f"position {position} outside the cache's {self.kv_rows} rows")
+        if self.kv_dtype == "q4" and position != 0 and self._evicted:
+            raise ValueError("rows have been evicted: reset() and feed the tokens again")
+        super().set_position(position)
+        if self.kv_dtype == "q4":
+            self._set_rows(np.full(self.B, position, dtype=np.int64))
+
+    def _set_rows(self, rows: np.ndarray) -> None:
+        self._rows = rows
+        self._evicted = self._evicted and bool(rows.any())
+        self._upload(self.ids["len"], rows.astype(np.float32))
+
+    _evicted = False         # cached rows are no longer the first positions
+
+    def _take_rows(self, tokens) -> None:
+        """Room for `tokens` new rows (of every sequence, or one number each) in a 4-bit cache: evict where they would not fit, then count them."""
+        if self.kv_dtype != "q4":
+            return
+        need = np.broadcast_to(np.asarray(tokens, dtype=np.int64), (self.B,))
+        if np.any(self._rows + need > self.kv_rows):
+            if self.kv_budget is None:
+                raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+            I, s = self.ids, []
+            for l in range(self.cfg.n_layers):
+                seen = I[f"seen.{l}"]
+                s += [OP_KV_EVICT_Q4, I["kv"], I["kv"], l, I["len"], seen, self.kv_budget, self.kv_recent, self.B, seen, I["len_kept"], -1]
+            s = np.asarray(s + [OP_COPY, I["len_kept"], 0, I["len"], 0, self.B], dtype=np.int32)
+            _lib.check(self.lib.deepj_cuda_flush_ops_async(s.ctypes.data, s.size))
+            self._evicted = self._evicted or bool(np.any(self._rows > self.kv_budget))
+            self._rows = np.minimum(self._rows, self.kv_budget)
+            if np.any(self._rows + need > self.kv_rows):
+                raise ValueError("more tokens at once than the cache has rows behind its budget")
+        self._rows = self._rows + need
+
+    def prefill_packed(self, prompts) -> np.ndarray:
+        """Feed prompts of different lengths, one per sequence (each at least one token), behind whatever the sequences hold; returns the greedy
+        pick after each one's last token.  All tokens of a pass run as packed rows: no row is padding.  Needs the 4-bit cache."""
+        if self.kv_dtype != "q4":
+            raise ValueError("packed prompts need kv_dtype 'q4'")
+        if self.tp_world > 1:
+            raise ValueError("packed prompts run on one GPU")
+        toks = [np.asarray(p, dtype=np.int64).reshape(-1) for p in prompts]
+        if len(toks) != self.B or any(t.size == 0 for t in toks):
+            raise ValueError(f"expected {self.B} prompts of at least one token")
+        if not self.loaded:
+            raise RuntimeError("weights are not loaded")
+        pos = self._download(self.ids["pos"], self.B).astype(np.int64)
+        for b, t in enumerate(toks):
+            if np.any(t < 0) or np.any(t >= self.cfg.vocab_size):
+                raise ValueError(f"Token id out of range: {int(t[(t < 0) | (t >= self.cfg.vocab_size)][0])}")
+            if pos[b] + t.size > self.cfg.max_seq_len:
+                raise ValueError(f"seqLen {int(pos[b]) + t.size} exceeds maxSeqLen {self.cfg.max_seq_len}")
+        longest = max(t.size for t in toks)
+        if self.kv_budget is None and any(self._rows[b] + t.size > self.kv_rows for b, t in enumerate(toks)):
+            raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+        C = min(self._chunk_tokens(), longest)
+        self._ensure_prefill_buffers(C)
+        P, I = self._prefill_ids, self.ids
+        for lo in range(0, longest, C):
+            parts = [t[lo:lo + C] for t in toks]
+            new = np.asarray([t.size for t in parts], dtype=np.int64)
+            starts = np.concatenate(([0], np.cumsum(new)))
+            ends = [(b, int(starts[b + 1]) - 1) for b in range(self.B) if new[b] > 0 and lo + C >= toks[b].size]
+            self._take_rows(new)
+            self._upload(P["tok"], np.concatenate(parts).astype(np.float32))
+            self._upload(P["starts"], starts)
+            if self.cfg.kind == "gpt":
+                self._upload(P["ppos"], np.concatenate([np.arange(pos[b], pos[b] + new[b]) for b in range(self.B)]))
+            st = self._build_prefill(0, ends, int(starts[-1]))
+            _lib.check(self.lib.deepj_cuda_flush_ops(st.ctypes.data, st.size))
+            pos += new
+            self._upload(I["pos"], pos.astype(np.float32))
+            self._upload(I["len"], self._rows.astype(np.float32))
+        self.position = int(pos.max())
+        hs = self._head_stream()
+        _lib.check(self.lib.deepj_cuda_flush_ops(hs.ctypes.data, hs.size))
+        return self.next_tokens()

@@ -73,6 +73,9 @@ class StreamDecoder:
         """Token ids [B × T] of the next chunk (row b·T + t)."""
         self._upload(self._prefill_ids["tok"], tokens.astype(np.float32).reshape(-1))
 
+    def _take_rows(self, tokens: int) -> None:
+        """Called before `tokens` new tokens of every sequence run: a cache that fills up makes room here."""
+
     # ── id / buffer helpers ──
     def _new_id(self) -> int:
         i = self._next_id
@@ -162,6 +165,7 @@ class StreamDecoder:
             raise ValueError(f"seqLen {self.position + 1} exceeds maxSeqLen {self.cfg.max_seq_len}")
         host, _ = self._streams()
         self.set_tokens(tokens)
+        self._take_rows(1)
         # enqueue the stream behind the upload and let the download's synchronisation be the only one of the step
         _lib.check(self.lib.deepj_cuda_flush_ops_async(host.ctypes.data, host.size))
         self.position += 1
@@ -175,6 +179,7 @@ class StreamDecoder:
             raise ValueError(f"seqLen {self.position + n_steps} exceeds maxSeqLen {self.cfg.max_seq_len}")
         _, dev = self._streams()
         for _ in range(n_steps):
+            self._take_rows(1)
             _lib.check(self.lib.deepj_cuda_flush_ops_async(dev.ctypes.data, dev.size))
         self.position += n_steps
         if sync:
@@ -207,6 +212,7 @@ class StreamDecoder:
                 self._prefill_streams.clear()
             self._prefill_streams[T] = self._build_prefill(T)
         st = self._prefill_streams[T]
+        self._take_rows(T)
         self._upload_chunk(p)
         _lib.check(self.lib.deepj_cuda_flush_ops(st.ctypes.data, st.size))
         self.position += T
@@ -318,6 +324,7 @@ class StreamDecoder:
             else:
                 if self.position + 1 > c.max_seq_len:
                     raise ValueError(f"seqLen {self.position + 1} exceeds maxSeqLen {c.max_seq_len}")
+                self._take_rows(1)
                 self._upload(I["tok"], np.asarray([out[-1]], dtype=np.float32))
                 _lib.check(self.lib.deepj_cuda_flush_ops(step.ctypes.data, step.size))
                 self.position += 1
@@ -350,6 +357,7 @@ class StreamDecoder:
         if not self.loaded:
             raise RuntimeError("weights are not loaded")
         host = self._build(feed_back=False)
+        self._take_rows(1)
         n = len(self._op_labels) + 1
         ms = np.zeros(n, dtype=np.float32)
         cnt = ctypes.c_int32(0)
