@@ -75,7 +75,7 @@ template <int NB> __device__ __forceinline__ void lds_scales(float (&s)[NB], con
 
 template <int NB, int HPB> struct DecodeShape {
     static constexpr int HD = 32 * NB, NT = (HPB + 1) / 2;
-    static constexpr int kStages = NB == 4 ? 3 : NB == 2 ? 5 : 6;
+    static constexpr int kStages = NB == 4 ? 2 : NB == 2 ? 4 : 6;
     static constexpr int kRing = kDecWarps * kStages * Q4Page<NB>::kBytes;
     static constexpr int kDigits = NB * HPB * 96;                        // of a warp: [block][head][digit][32 rows]
     static constexpr size_t kSmem = kRing + kDecWarps * kDigits + 64;    // 64: zeros for the columns without a head

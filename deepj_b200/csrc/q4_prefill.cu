@@ -5,11 +5,11 @@
 //   S = Q·Kᵀ    Q in fp16 halves hi + lo of the rotated row times a power of two (22 bits); a stored key, code · scale, is exact in fp16: two MMAs
 //   P = 2^(S·c − m) per row, in halves hi + lo again, written over S in tensor memory, from where it is the A operand of
 //   O += P·V    with O in tensor memory as well
-//   warps 0-3   a thread is a row: running maximum and sum of the softmax in fp32, no exchange between lanes.  O is multiplied by the change of the
+//   warps 0-7   two threads to a row: running maximum and sum of the softmax in fp32, no exchange between lanes.  O is multiplied by the change of the
 //               maximum only when that grew by more than 2^8: until then P is larger than one, which fp16 and the fp32 sums have room for
-//   warps 4-7   a warp is a page: 4-bit codes → fp16 tiles with 128-byte swizzle, keys a tile ahead of the values
-//   warp 8      one thread brings the pages' halves with bulk copies into a ring
-//   warp 9      one thread issues the MMAs: Q·K of the next tile before P·V of this one, so that the softmax never waits for them
+//   warps 8-11  a warp is a page: 4-bit codes → fp16 tiles with 128-byte swizzle, keys a tile ahead of the values
+//   warp 12     one thread brings the pages' halves with bulk copies into a ring
+//   warp 13     one thread issues the MMAs: Q·K of the next tile before P·V of this one, so that the softmax never waits for them
 // Tensor memory: three S/P buffers of 128 columns and O.  Every wait is bounded (codes 341-349 in the device error word).
 #include <algorithm>
 #include <cmath>
@@ -23,7 +23,7 @@ namespace dj {
 namespace {
 
 constexpr int kPT = 128;                          // query rows and keys of a tile
-constexpr int kPThreads = 320;
+constexpr int kPThreads = 448;                    // warps: 8 softmax, 4 conversion, copies, MMAs
 constexpr int kPRing = 3;                         // ring stages: the K or the V halves of a tile's four pages
 
 struct PrefillParams {
@@ -81,19 +81,21 @@ __device__ __forceinline__ uint2 codes_to_half(uint32_t nibbles, __half2 scale) 
 // Row `lane` of a page's K or V half → row `row` of an fp16 tile, 16 bytes (8 dims) a time.
 template <int NB>
 __device__ __forceinline__ void convert_row(const unsigned char* half, int lane, unsigned char* tile, int row) {
-    uint32_t w[4][NB];
+    __half2 scale[NB];
 #pragma unroll
-    for (int t = 0; t < 4; t++) piece_of<NB>(w[t], half + Q4Page<NB>::word(lane, t, 0));
+    for (int j = 0; j < NB; j++)
+        scale[j] = __float2half2_rn(__uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(half + Q4Page<NB>::kKs + (lane * NB + j) * 2) << 16));
+#pragma unroll 1
+    for (int u = 0; u < 2; u++) {                 // rolled: the roles of a block run side by side and share the instruction cache
+        uint32_t w[2][NB];
+        piece_of<NB>(w[0], half + Q4Page<NB>::word(lane, 2 * u, 0));
+        piece_of<NB>(w[1], half + Q4Page<NB>::word(lane, 2 * u + 1, 0));
 #pragma unroll
-    for (int j = 0; j < NB; j++) {
-        const float s = __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(half + Q4Page<NB>::kKs + (lane * NB + j) * 2) << 16);
-        const __half2 scale = __float2half2_rn(s);
+        for (int j = 0; j < NB; j++)
 #pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t a = ((w[2 * u][j] >> (4 * x)) & 0x0f0f0f0fu) ^ 0x08080808u, b = ((w[2 * u + 1][j] >> (4 * x)) & 0x0f0f0f0fu) ^ 0x08080808u;
-                const uint2 lo = codes_to_half(a, scale), hi = codes_to_half(b, scale);
+            for (int x = 0; x < 2; x++) {
+                const uint32_t a = ((w[0][j] >> (4 * x)) & 0x0f0f0f0fu) ^ 0x08080808u, b = ((w[1][j] >> (4 * x)) & 0x0f0f0f0fu) ^ 0x08080808u;
+                const uint2 lo = codes_to_half(a, scale[j]), hi = codes_to_half(b, scale[j]);
                 const int c = 4 * j + 2 * x + u;
                 *reinterpret_cast<uint4*>(tile + (c >> 3) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
@@ -180,6 +182,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
     __shared__ __align__(8) unsigned long long s_bar[2 * kPRing + 8 + 6 + 1];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
+    __shared__ float s_max[2][kPT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
@@ -196,12 +199,12 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
     if (tid == 0) {
         for (int s = 0; s < kPRing; s++) { mbar_init(ringFull(s), 1); mbar_init(ringEmpty(s), 4); }
         for (int s = 0; s < 2; s++) { mbar_init(kFull(s), 4); mbar_init(kEmpty(s), 1); mbar_init(vFull(s), 4); mbar_init(vEmpty(s), 1); }
-        for (int s = 0; s < 3; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 4); }
+        for (int s = 0; s < 3; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 8); }
         mbar_init(qReady, 4);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
+    if (warp == 13) tmem_alloc(smem_u32(&s_tmem), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -218,41 +221,53 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
     const int used = max(0, min(tokensPerTile, room - t0));              // tokens of this tile
     const int keys = used > 0 ? len + t0 + used : 0, tiles = (keys + kPT - 1) / kPT, pages = (keys + kQ4Page - 1) / kQ4Page;
 
-    if (warp < 4) {
-        const int row = tid, token = row / p.ratio, head = g * p.ratio + row % p.ratio;
+    if (warp < 8) {
+        // two threads to a row, 64 keys of a tile each: warps w and w + 4 exchange what they find through shared memory
+        const int part = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, token = row / p.ratio, head = g * p.ratio + row % p.ratio;
         const bool on = token < used;
         const int m = first + t0 + token, last = on ? len + t0 + token : -1;      // the row's place in the buffers, its newest key
+        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
         float c = 1.0f, top = -INFINITY, sum = 0.0f;
         if (tiles > 0) {
-            c = query_row<NB>(p, m, head, pos + t0 + token, on, smem, smem + S::kTile, row);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(qReady);
+            if (part == 0) {
+                s_max[0][row] = c = query_row<NB>(p, m, head, pos + t0 + token, on, smem, smem + S::kTile, row);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(qReady);
+            }
+            meet();
+            c = s_max[0][row];
+            meet();
         }
-        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
         for (int j = 0; j < tiles; j++) {
-            if (!__all_sync(0xffffffffu, mbar_wait(sFull(j % 3), (j / 3) & 1, &s_abort, p.error, 341))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, mbar_wait(sFull(j % 3), (j / 3) & 1, &s_abort, p.error, 341))) ok = false;
             tc_fence_after();
-            uint32_t v[128];
-            tmem_ld128(mine + (uint32_t)(j % 3 * kPT), v);
-            if (!__all_sync(0xffffffffu, last >= j * kPT + kPT - 1)) {   // the tile reaches past a row's newest key
+            uint32_t v[64];
+            const uint32_t at = mine + (uint32_t)(j % 3 * kPT + part * 64);
+            tmem_ld64(at, v);
+            const int left = last - j * kPT - part * 64;                 // newest key within these 64
+            if (!__all_sync(0xffffffffu, left >= 63)) {
 #pragma unroll
-                for (int k = 0; k < 128; k++)
-                    if (j * kPT + k > last) v[k] = 0xff800000u;
+                for (int k = 0; k < 64; k++)
+                    if (k > left) v[k] = 0xff800000u;
             }
             float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < 128; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
-            const float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+            for (int k = 0; k < 64; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
+            float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+            s_max[part][row] = most;
+            meet();
+            most = fmaxf(most, s_max[1 - part][row]);
             const bool grown = most > top + 8.0f;                        // also the first keys of a row
-            if (__any_sync(0xffffffffu, grown)) {
+            if (__any_sync(0xffffffffu, grown)) {                        // both warps of a row come to the same
                 const float now = grown ? most : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
                 if (j > 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(vEmpty((j - 1) & 1), ((j - 1) >> 1) & 1, &s_abort, p.error, 342))) { ok = false; break; }
+                    if (!__all_sync(0xffffffffu, mbar_wait(vEmpty((j - 1) & 1), ((j - 1) >> 1) & 1, &s_abort, p.error, 342))) ok = false;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int k = 0; k < HD; k += 32) {
+                    for (int k = 32 * part; k < HD; k += 64) {
                         uint32_t o[32];
                         tmem_ld32(mine + kO + k, o);
 #pragma unroll
@@ -265,25 +280,35 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
             }
             const float shift = top > -INFINITY ? -top : 0.0f;           // a row without keys yet: every weight is 2^-inf
             float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            uint32_t w[128];
 #pragma unroll
-            for (int k = 0; k < 64; k++) {
-                const float x = ex2(fmaf(__uint_as_float(v[2 * k]), c, shift)), y = ex2(fmaf(__uint_as_float(v[2 * k + 1]), c, shift));
-                s4[k & 3] += x + y;
-                split_half(x, y, w[k], w[64 + k]);
+            for (int q = 0; q < 2; q++) {
+                uint32_t w[32];
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float x = ex2(fmaf(__uint_as_float(v[32 * q + 2 * k]), c, shift)), y = ex2(fmaf(__uint_as_float(v[32 * q + 2 * k + 1]), c, shift));
+                    s4[k & 3] += x + y;
+                    split_half(x, y, w[k], w[16 + k]);
+                }
+                tmem_st32(at + q * 32, w);                               // 32 keys: sixteen columns hi, sixteen lo
             }
             sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
-            tmem_st128(mine + (uint32_t)(j % 3 * kPT), w);
+            tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pReady(j % 3));
+            meet();                                                      // the maxima are read
         }
-        if (ok && tiles > 0 && __all_sync(0xffffffffu, mbar_wait(vEmpty((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, &s_abort, p.error, 343))) {
+        if (tiles > 0) {
+            s_max[part][row] = sum;
+            meet();
+            sum += s_max[1 - part][row];
+        }
+        if (tiles > 0 && __all_sync(0xffffffffu, ok && mbar_wait(vEmpty((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, &s_abort, p.error, 343))) {
             tc_fence_after();
             const float inv = 1.0f / sum;
             float* const to = p.out + (size_t)m * p.ldo + head * HD;
 #pragma unroll 1
-            for (int k = 0; k < HD; k += 32) {
+            for (int k = 32 * part; k < HD; k += 64) {
                 uint32_t o[32];
                 tmem_ld32(mine + kO + k, o);
                 if (on)
@@ -292,10 +317,11 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
                         *reinterpret_cast<float4*>(to + k + i) = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv,
                                                                             __uint_as_float(o[i + 3]) * inv);
             }
-            if (on && p.stats != nullptr && t0 + token >= room - p.window) *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
+            if (part == 0 && on && p.stats != nullptr && t0 + token >= room - p.window)
+                *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
         }
-    } else if (warp < 8) {
-        const int w = warp - 4;                   // page of the tile
+    } else if (warp < 12) {
+        const int w = warp - 8;                   // page of the tile
         bool ok = true;
         int item = 0;
         auto convert = [&](int j, bool value) {
@@ -315,7 +341,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
             if (j < tiles) ok = convert(j, false);
             if (ok && j > 0) ok = convert(j - 1, true);
         }
-    } else if (warp == 8) {
+    } else if (warp == 12) {
         if (lane == 0) {
             const unsigned char* const plane = p.cache + ((size_t)b * p.G + g) * p.pages * Q4Page<NB>::kBytes;
             int item = 0;
@@ -368,7 +394,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int k = 0; k < kPT / 16; k++) umma_f16_ta(tmem + kO, a + h * 64 + k * 8, desc_mn(v0 + k * 2048), kIdescPV, (j | h | k) != 0);
+                    for (int k = 0; k < kPT / 16; k++) umma_f16_ta(tmem + kO, a + (k >> 1) * 32 + h * 16 + (k & 1) * 8, desc_mn(v0 + k * 2048), kIdescPV, (j | h | k) != 0);
                 umma_commit(vEmpty(j & 1));
             }
         }
@@ -376,7 +402,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+    if (warp == 13) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 // ───────────── weights of the last tokens ─────────────
