@@ -7,9 +7,9 @@
 //   O += P·V    with O in tensor memory as well
 //   warps 0-7   two threads to a row: running maximum and sum of the softmax in fp32, no exchange between lanes.  O is multiplied by the change of the
 //               maximum only when that grew by more than 2^8: until then P is larger than one, which fp16 and the fp32 sums have room for
-//   warps 8-11  a warp is a page: 4-bit codes → fp16 tiles with 128-byte swizzle, keys a tile ahead of the values
-//   warp 12     one thread brings the pages' halves with bulk copies into a ring
-//   warp 13     one thread issues the MMAs: Q·K of the next tile before P·V of this one, so that the softmax never waits for them
+//   warps 8-15  two warps are a page: 4-bit codes → fp16 tiles with 128-byte swizzle, keys a tile ahead of the values
+//   warp 16     one thread brings the pages' halves with bulk copies into a ring
+//   warp 17     one thread issues the MMAs: Q·K of the next tile before P·V of this one, so that the softmax never waits for them
 // Tensor memory: three S/P buffers of 128 columns and O.  Every wait is bounded (codes 341-349 in the device error word).
 #include <algorithm>
 #include <cmath>
@@ -23,7 +23,7 @@ namespace dj {
 namespace {
 
 constexpr int kPT = 128;                          // query rows and keys of a tile
-constexpr int kPThreads = 448;                    // warps: 8 softmax, 4 conversion, copies, MMAs
+constexpr int kPThreads = 576;                    // warps: 8 softmax, 8 conversion, copies, MMAs
 constexpr int kPRing = 3;                         // ring stages: the K or the V halves of a tile's four pages
 
 struct PrefillParams {
@@ -70,80 +70,106 @@ template <int NB> __device__ __forceinline__ void piece_of(uint32_t (&w)[NB], co
     else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
-// Four codes in the low nibbles of a word's bytes, sign bits flipped (code + 8) → four fp16 values: 1024 + 8 + code, minus 1032, times the scale; all exact.
-__device__ __forceinline__ uint2 codes_to_half(uint32_t nibbles, __half2 scale) {
-    const uint32_t a = __byte_perm(nibbles, 0x64646464u, 0x4140), b = __byte_perm(nibbles, 0x64646464u, 0x4342);
-    const __half2 off = __float2half2_rn(1032.0f);
-    const __half2 x = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&a), off), scale), y = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&b), off), scale);
-    return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+// A tile's row has its dims in the order in which a page word gives them: 16 bytes are word (t, j), its values dims 32j + 4t + {0, 2, 16, 18, 1, 3, 17, 19}.
+// Queries are laid down in the same order; outputs are put back when they are stored.
+// Bits 6 … 9 of a half of 16 + u are u, the code + 8: (word moved & 0x03c0) ^ 0x4e00 = 24 + code, and (24 + code)·scale - 24·scale = code · scale in one
+// fused operation.  24·scale has 10 bits; where it would leave fp16 (scales above 2729) the code is formed first.
+__device__ __forceinline__ uint32_t half_of(uint32_t moved, __half2 scale, __half2 off, bool wide) {
+    const uint32_t x = (moved & 0x03c003c0u) ^ 0x4e004e00u;
+    const __half2 v = *reinterpret_cast<const __half2*>(&x);
+    const __half2 r = wide ? __hmul2(__hsub2(v, __float2half2_rn(24.0f)), scale) : __hfma2(v, scale, off);
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
-
-// Row `lane` of a page's K or V half → row `row` of an fp16 tile, 16 bytes (8 dims) a time.
-template <int NB>
-__device__ __forceinline__ void convert_row(const unsigned char* half, int lane, unsigned char* tile, int row) {
-    __half2 scale[NB];
+template <int NB, bool WIDE>
+__device__ __forceinline__ void convert_words(const unsigned char* half, int lane, unsigned char* tile, int row, const __half2 (&scale)[NB], int t0, int t1) {
+    __half2 off[NB];
 #pragma unroll
-    for (int j = 0; j < NB; j++)
-        scale[j] = __float2half2_rn(__uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(half + Q4Page<NB>::kKs + (lane * NB + j) * 2) << 16));
+    for (int j = 0; j < NB; j++) off[j] = __hmul2(scale[j], __float2half2_rn(-24.0f));
 #pragma unroll 1
-    for (int u = 0; u < 2; u++) {                 // rolled: the roles of a block run side by side and share the instruction cache
-        uint32_t w[2][NB];
-        piece_of<NB>(w[0], half + Q4Page<NB>::word(lane, 2 * u, 0));
-        piece_of<NB>(w[1], half + Q4Page<NB>::word(lane, 2 * u + 1, 0));
+    for (int t = t0; t < t1; t++) {               // rolled: the roles of a block run side by side and share the instruction cache
+        uint32_t w[NB];
+        piece_of<NB>(w, half + Q4Page<NB>::word(lane, t, 0));
 #pragma unroll
-        for (int j = 0; j < NB; j++)
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const uint32_t a = ((w[0][j] >> (4 * x)) & 0x0f0f0f0fu) ^ 0x08080808u, b = ((w[1][j] >> (4 * x)) & 0x0f0f0f0fu) ^ 0x08080808u;
-                const uint2 lo = codes_to_half(a, scale[j]), hi = codes_to_half(b, scale[j]);
-                const int c = 4 * j + 2 * x + u;
-                *reinterpret_cast<uint4*>(tile + (c >> 3) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
+        for (int j = 0; j < NB; j++) {
+            const int c = 4 * j + t;
+            *reinterpret_cast<uint4*>(tile + (j >> 1) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                make_uint4(half_of(w[j] << 6, scale[j], off[j], WIDE), half_of(w[j] << 2, scale[j], off[j], WIDE), half_of(w[j] >> 2, scale[j], off[j], WIDE),
+                           half_of(w[j] >> 6, scale[j], off[j], WIDE));
+        }
     }
 }
+// Row `lane` of a page's K or V half, its words (t0 … t1 - 1, j) → row `row` of an fp16 tile.
 template <int NB>
-__device__ __forceinline__ void zero_row(unsigned char* tile, int row) {
+__device__ __forceinline__ void convert_row(const unsigned char* half, int lane, unsigned char* tile, int row, int t0, int t1) {
+    __half2 scale[NB];
+    float most = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4 * NB; c++) *reinterpret_cast<uint4*>(tile + (c >> 3) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < NB; j++) {
+        const float s = __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(half + Q4Page<NB>::kKs + (lane * NB + j) * 2) << 16);
+        most = fmaxf(most, s);
+        scale[j] = __float2half2_rn(s);
+    }
+    if (__any_sync(0xffffffffu, most > 2048.0f)) convert_words<NB, true>(half, lane, tile, row, scale, t0, t1);
+    else convert_words<NB, false>(half, lane, tile, row, scale, t0, t1);
+}
+template <int NB>
+__device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, int t1) {
+#pragma unroll 1
+    for (int c = 0; c < 4 * NB; c++)
+        if ((c & 3) >= t0 && (c & 3) < t1) *reinterpret_cast<uint4*>(tile + (c >> 3) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
 }
 
-// A query row, rotated at `position`, in halves of fp16 times a power of two → tile row `row`; returns the factor that makes a sum of products a score
-// in log2 units (NaN where the row holds an infinity or a NaN).
-template <int NB>
-__device__ __forceinline__ float query_row(const PrefillParams& p, int m, int head, int position, bool on, unsigned char* hi, unsigned char* lo, int row) {
-    constexpr int HD = 32 * NB;
-    float4 x[HD / 4];
-    const float* const q = p.qkv + (size_t)m * p.ld + p.q_off + head * HD;
-    const float* const cs = p.cosT + (size_t)position * (HD / 2);
-    const float* const sn = p.sinT + (size_t)position * (HD / 2);
-    float most = 0.0f, bad = 0.0f;
+// Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 8·NB lanes of four values each; `place(row, m, head, position)` says
+// which one row `row` is (false: zeros).  factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).
+template <int NB, typename Place>
+__device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, Place place) {
+    constexpr int HD = 32 * NB, LPR = 8 * NB, RPW = 32 / LPR;
+    const int e = lane % LPR;
+    // this lane's dims 4e … 4e + 3 in the tiles' order: (0, 2) and (1, 3), eight bytes apart
+    const int piece = (e >> 3) * 4 + (e & 3), at = (piece >> 3) * (kPT * 128) + (e & 4);
+#pragma unroll 4
+    for (int r = warp * RPW + lane / LPR; r < kPT; r += warps * RPW) {
+        int m, head, position;
+        const bool on = place(r, m, head, position);
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (on) {
+            const size_t tab = (size_t)position * (HD / 2) + 2 * e;
+            x = q4_rotate(*reinterpret_cast<const float4*>(p.qkv + (size_t)m * p.ld + p.q_off + head * HD + 4 * e), *reinterpret_cast<const float2*>(p.cosT + tab),
+                          *reinterpret_cast<const float2*>(p.sinT + tab));
+        }
+        float most = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), bad = (x.x + x.y + x.z + x.w) * 0.0f;
 #pragma unroll
-    for (int i = 0; i < HD / 4; i++) {
-        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (on) x[i] = q4_rotate(*reinterpret_cast<const float4*>(q + 4 * i), *reinterpret_cast<const float2*>(cs + 2 * i), *reinterpret_cast<const float2*>(sn + 2 * i));
+        for (int o = 1; o < LPR; o <<= 1) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o)); bad += __shfl_xor_sync(0xffffffffu, bad, o); }
+        // the largest value comes to 256 … 512
+        most = fmaxf(most, 7.8886091e-31f);
+        const int bits = __float_as_int(most) & 0x7f800000;
+        const bool fine = bad == 0.0f && most < 1e30f;
+        const float mul = fine ? __int_as_float(0x7f000000 - bits) * 256.0f : 0.0f;
+        if (!fine) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        uint2 h, l;
+        split_half(x.x * mul, x.z * mul, h.x, l.x);
+        split_half(x.y * mul, x.w * mul, h.y, l.y);
+        const int to = at + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint32_t*>(hi + to) = h.x; *reinterpret_cast<uint32_t*>(hi + to + 8) = h.y;
+        *reinterpret_cast<uint32_t*>(lo + to) = l.x; *reinterpret_cast<uint32_t*>(lo + to + 8) = l.y;
+        if (e == 0) factors[r] = fine ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
     }
-#pragma unroll
-    for (int i = 0; i < HD / 4; i++) {
-        most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
-        bad += (x[i].x + x[i].y + x[i].z + x[i].w) * 0.0f;
-    }
-    // the largest value comes to 256 … 512
-    const bool some = most > 7.8886091e-31f && most < 1e30f;
-    const int bits = some ? __float_as_int(most) & 0x7f800000 : 0x3f800000;
-    const float mul = bad == 0.0f && some ? __int_as_float(0x7f000000 - bits) * 256.0f : 0.0f;
-#pragma unroll
-    for (int c = 0; c < HD / 8; c++) {
-        const float4 a = x[2 * c], b = x[2 * c + 1];
-        uint4 h, l;
-        split_half(a.x * mul, a.y * mul, h.x, l.x); split_half(a.z * mul, a.w * mul, h.y, l.y);
-        split_half(b.x * mul, b.y * mul, h.z, l.z); split_half(b.z * mul, b.w * mul, h.w, l.w);
-        if (mul == 0.0f) h = l = make_uint4(0, 0, 0, 0);
-        const int at = (c >> 3) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(hi + at) = h;
-        *reinterpret_cast<uint4*>(lo + at) = l;
-    }
-    return __int_as_float(bits) * (1.0f / 256.0f) * p.scale + (some || most == 0.0f || bad != 0.0f ? bad : most < 1.0f ? 0.0f : __int_as_float(0x7fc00000));
 }
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
 // Sequence and first token of query tile `tile`, the last tile of a sequence first; whole warps call it.
 __device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int tokensPerTile, int lane, int& b, int& first, int& tokens, int& t0) {
@@ -179,32 +205,32 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
     constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);      // B MN-major
     constexpr uint32_t kO = 3 * kPT;              // O's first column
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long s_bar[2 * kPRing + 8 + 6 + 1];
+    __shared__ __align__(8) unsigned long long s_bar[2 * kPRing + 14];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
-    __shared__ float s_max[2][kPT];
+    __shared__ float s_max[2][2][kPT], s_factor[kPT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
     auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
     auto ringFull = [&](int s) { return bar(s); };
     auto ringEmpty = [&](int s) { return bar(kPRing + s); };
-    auto kFull = [&](int s) { return bar(2 * kPRing + s); };
-    auto kEmpty = [&](int s) { return bar(2 * kPRing + 2 + s); };
-    auto vFull = [&](int s) { return bar(2 * kPRing + 4 + s); };
-    auto vEmpty = [&](int s) { return bar(2 * kPRing + 6 + s); };        // P·V of a tile is done
-    auto sFull = [&](int s) { return bar(2 * kPRing + 8 + s); };
-    auto pReady = [&](int s) { return bar(2 * kPRing + 11 + s); };
-    const uint32_t qReady = bar(2 * kPRing + 14);
+    auto kEmpty = [&](int s) { return bar(2 * kPRing + s); };           // Q·K of a tile is done
+    auto vFull = [&](int s) { return bar(2 * kPRing + 2 + s); };         // the values of a tile stand, and so do the keys of the next one
+    auto vEmpty = [&](int s) { return bar(2 * kPRing + 4 + s); };        // P·V of a tile is done
+    auto sFull = [&](int s) { return bar(2 * kPRing + 6 + s); };
+    auto pReady = [&](int s) { return bar(2 * kPRing + 9 + s); };
+    const uint32_t qReady = bar(2 * kPRing + 12), firstKeys = bar(2 * kPRing + 13);
     if (tid == 0) {
-        for (int s = 0; s < kPRing; s++) { mbar_init(ringFull(s), 1); mbar_init(ringEmpty(s), 4); }
-        for (int s = 0; s < 2; s++) { mbar_init(kFull(s), 4); mbar_init(kEmpty(s), 1); mbar_init(vFull(s), 4); mbar_init(vEmpty(s), 1); }
+        for (int s = 0; s < kPRing; s++) { mbar_init(ringFull(s), 1); mbar_init(ringEmpty(s), 8); }
+        for (int s = 0; s < 2; s++) { mbar_init(kEmpty(s), 1); mbar_init(vFull(s), 8); mbar_init(vEmpty(s), 1); }
         for (int s = 0; s < 3; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 8); }
-        mbar_init(qReady, 4);
+        mbar_init(qReady, 8);
+        mbar_init(firstKeys, 8);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 13) tmem_alloc(smem_u32(&s_tmem), 512);
+    if (warp == 17) tmem_alloc(smem_u32(&s_tmem), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -227,39 +253,50 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
         const bool on = token < used;
         const int m = first + t0 + token, last = on ? len + t0 + token : -1;      // the row's place in the buffers, its newest key
         auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
-        float c = 1.0f, top = -INFINITY, sum = 0.0f;
+        float c = 1.0f, top = -INFINITY;
+        float2 sums = make_float2(0.0f, 0.0f);
         if (tiles > 0) {
-            if (part == 0) {
-                s_max[0][row] = c = query_row<NB>(p, m, head, pos + t0 + token, on, smem, smem + S::kTile, row);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(qReady);
-            }
-            meet();
-            c = s_max[0][row];
-            meet();
+            query_rows<NB>(p, warp, 8, lane, smem, smem + S::kTile, s_factor, [&](int r, int& qm, int& qh, int& qp) {
+                const int t = r / p.ratio;
+                qm = first + t0 + t; qh = g * p.ratio + r - t * p.ratio; qp = pos + t0 + t;
+                return t < used;
+            });
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qReady);
+            asm volatile("bar.sync 5, 256;" ::: "memory");
+            c = s_factor[row];
         }
         const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
         bool ok = true;
         for (int j = 0; j < tiles; j++) {
             if (!__all_sync(0xffffffffu, mbar_wait(sFull(j % 3), (j / 3) & 1, &s_abort, p.error, 341))) ok = false;
             tc_fence_after();
-            uint32_t v[64];
             const uint32_t at = mine + (uint32_t)(j % 3 * kPT + part * 64);
-            tmem_ld64(at, v);
             const int left = last - j * kPT - part * 64;                 // newest key within these 64
-            if (!__all_sync(0xffffffffu, left >= 63)) {
+            const bool cut = !__all_sync(0xffffffffu, left >= 63);
+            float most = -INFINITY;
+            // columns are read twice, 32 a time, rather than kept: less code and registers for a load that takes 50 cycles
+            auto columns = [&](int q, uint32_t (&v)[32]) {
+                tmem_ld32(at + q * 32, v);
+                if (cut)
 #pragma unroll
-                for (int k = 0; k < 64; k++)
-                    if (k > left) v[k] = 0xff800000u;
+                    for (int k = 0; k < 32; k++)
+                        if (k > left - q * 32) v[k] = 0xff800000u;
+            };
+#pragma unroll 1
+            for (int q = 0; q < 2; q++) {
+                uint32_t v[32];
+                columns(q, v);
+                float m2[2] = {most, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) m2[(k >> 1) & 1] = max3(m2[(k >> 1) & 1], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                most = fmaxf(m2[0], m2[1]);
             }
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int k = 0; k < 64; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
-            float most = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
-            s_max[part][row] = most;
+            most *= c;
+            s_max[j & 1][part][row] = most;
             meet();
-            most = fmaxf(most, s_max[1 - part][row]);
+            most = fmaxf(most, s_max[j & 1][1 - part][row]);
             const bool grown = most > top + 8.0f;                        // also the first keys of a row
             if (__any_sync(0xffffffffu, grown)) {                        // both warps of a row come to the same
                 const float now = grown ? most : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
@@ -275,73 +312,89 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
                         tmem_st32(mine + kO + k, o);
                     }
                 }
-                sum *= f;
+                sums.x *= f; sums.y *= f;
                 top = now;
             }
             const float shift = top > -INFINITY ? -top : 0.0f;           // a row without keys yet: every weight is 2^-inf
-            float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+            const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift), minus = make_float2(-1.0f, -1.0f);
+#pragma unroll 1
             for (int q = 0; q < 2; q++) {
-                uint32_t w[32];
+                uint32_t v[32], w[32];
+                columns(q, v);
 #pragma unroll
                 for (int k = 0; k < 16; k++) {
-                    const float x = ex2(fmaf(__uint_as_float(v[32 * q + 2 * k]), c, shift)), y = ex2(fmaf(__uint_as_float(v[32 * q + 2 * k + 1]), c, shift));
-                    s4[k & 3] += x + y;
-                    split_half(x, y, w[k], w[16 + k]);
+                    const float2 x = fma2(make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])), c2, shift2);
+                    const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                    sums = add2(sums, e);
+                    // hi: the first 11 bits; the rest is exact
+                    const float2 hi = make_float2(__uint_as_float(__float_as_uint(e.x) & 0xffffe000u), __uint_as_float(__float_as_uint(e.y) & 0xffffe000u));
+                    const float2 lo = fma2(hi, minus, e);
+                    w[k] = half2_bits(hi.x, hi.y);
+                    w[16 + k] = half2_bits(lo.x, lo.y);
                 }
                 tmem_st32(at + q * 32, w);                               // 32 keys: sixteen columns hi, sixteen lo
             }
-            sum += (s4[0] + s4[1]) + (s4[2] + s4[3]);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pReady(j % 3));
-            meet();                                                      // the maxima are read
+        }
+        float sum = sums.x + sums.y;
+        if (tiles > 0) {
+            s_max[tiles & 1][part][row] = sum;
+            meet();
+            sum += s_max[tiles & 1][1 - part][row];
         }
         if (tiles > 0) {
-            s_max[part][row] = sum;
-            meet();
-            sum += s_max[1 - part][row];
-        }
-        if (tiles > 0 && __all_sync(0xffffffffu, ok && mbar_wait(vEmpty((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, &s_abort, p.error, 343))) {
+            // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(vEmpty((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, &s_abort, p.error, 343));
             tc_fence_after();
             const float inv = 1.0f / sum;
-            float* const to = p.out + (size_t)m * p.ldo + head * HD;
+            constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;
+            float* const stage = reinterpret_cast<float*>(smem);
 #pragma unroll 1
-            for (int k = 32 * part; k < HD; k += 64) {
+            for (int k = 32 * part; ok && k < HD; k += 64) {
                 uint32_t o[32];
                 tmem_ld32(mine + kO + k, o);
-                if (on)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(to + k + i) = make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv,
-                                                                            __uint_as_float(o[i + 3]) * inv);
+                for (int i = 0; i < 8; i++) {     // dims 4t … 4t + 3, 16 dims on for the high nibbles
+                    const int from = 8 * (i & 3) + 2 * (i >> 2);
+                    *reinterpret_cast<float4*>(stage + row * PITCH + k + 4 * i) =
+                        make_float4(__uint_as_float(o[from]) * inv, __uint_as_float(o[from + 4]) * inv, __uint_as_float(o[from + 1]) * inv, __uint_as_float(o[from + 5]) * inv);
+                }
+            }
+            asm volatile("bar.sync 5, 256;" ::: "memory");
+            for (int r = warp * RPW + lane / LPR; ok && r < used * p.ratio; r += 8 * RPW) {
+                const int t = r / p.ratio, e = lane % LPR;
+                *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) =
+                    *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
             }
             if (part == 0 && on && p.stats != nullptr && t0 + token >= room - p.window)
                 *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
         }
-    } else if (warp < 12) {
-        const int w = warp - 8;                   // page of the tile
+    } else if (warp < 16) {
+        const int w = warp & 3, t0 = (warp - 8) >> 2 << 1;               // page of the tile, half of a row's words
         bool ok = true;
         int item = 0;
-        auto convert = [&](int j, bool value) {
-            const uint32_t empty = value ? vEmpty(j & 1) : kEmpty(j & 1), full = value ? vFull(j & 1) : kFull(j & 1);
-            if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(empty, ((j >> 1) - 1) & 1, &s_abort, p.error, 344))) return false;
-            if (!__all_sync(0xffffffffu, mbar_wait(ringFull(item % kPRing), (item / kPRing) & 1, &s_abort, p.error, 345))) return false;
+#pragma unroll 1
+        for (int i = 0; i < 2 * tiles && ok; i++) {                      // K 0, K 1, V 0, K 2, V 1, …, V tiles - 1
+            const bool value = i > 0 && (i % 2 == 0 || i == 2 * tiles - 1);
+            const int j = i == 0 ? 0 : value ? (i - 1) / 2 : (i + 1) / 2;
+            if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(value ? vEmpty(j & 1) : kEmpty(j & 1), ((j >> 1) - 1) & 1, &s_abort, p.error, 344))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(ringFull(item % kPRing), (item / kPRing) & 1, &s_abort, p.error, 345))) break;
             unsigned char* const tile = smem + (value ? 4 + (j & 1) : 2 + (j & 1)) * S::kTile;
-            if (4 * j + w < pages) convert_row<NB>(smem + S::kRingAt + item % kPRing * S::kStage + w * Q4Page<NB>::kHalf, lane, tile, 32 * w + lane);
-            else if (value) zero_row<NB>(tile, 32 * w + lane);           // weights of 0 meet no garbage
+            if (4 * j + w < pages) convert_row<NB>(smem + S::kRingAt + item % kPRing * S::kStage + w * Q4Page<NB>::kHalf, lane, tile, 32 * w + lane, t0, t0 + 2);
+            else if (value) zero_row<NB>(tile, 32 * w + lane, t0, t0 + 2);      // weights of 0 meet no garbage
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(ringEmpty(item % kPRing)); mbar_arrive(full); }
+            if (lane == 0) {
+                mbar_arrive(ringEmpty(item % kPRing));
+                if (value) mbar_arrive(vFull(j & 1));
+                else if (j == 0) mbar_arrive(firstKeys);
+            }
             item++;
-            return true;
-        };
-        for (int j = 0; j <= tiles && ok; j++) {  // K 0, K 1, V 0, K 2, V 1, …
-            if (j < tiles) ok = convert(j, false);
-            if (ok && j > 0) ok = convert(j - 1, true);
         }
-    } else if (warp == 12) {
+    } else if (warp == 16) {
         if (lane == 0) {
             const unsigned char* const plane = p.cache + ((size_t)b * p.G + g) * p.pages * Q4Page<NB>::kBytes;
             int item = 0;
@@ -367,42 +420,49 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
         __syncwarp();
     } else {
         if (lane == 0 && tiles > 0) {
-            const uint32_t qh = base, ql = base + S::kTile;
+            // rolled: what one thread issues has to come from the instruction cache in time
             auto scores = [&](int j) {
-                if (!mbar_wait(kFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 347)) return false;
-                // P·V of tile j - 3 has read this buffer
-                if (j >= 3 && !mbar_wait(vEmpty((j - 3) & 1), ((j - 3) >> 1) & 1, &s_abort, p.error, 348)) return false;
-                tc_fence_after();
-                const uint32_t k0 = base + (2 + (j & 1)) * S::kTile, d = tmem + (uint32_t)(j % 3 * kPT);
-#pragma unroll
+                const uint32_t d = tmem + (uint32_t)(j % 3 * kPT);
+                const uint64_t q0 = desc_k(base), k0 = desc_k(base + (2 + (j & 1)) * S::kTile);
+#pragma unroll 1
                 for (int h = 0; h < 2; h++)
+#pragma unroll 1
+                    for (int c = 0; c < S::kChunks; c++) {
+                        const uint64_t a = q0 + (uint32_t)((h * S::kTile + c * (kPT * 128)) >> 4), b = k0 + (uint32_t)((c * (kPT * 128)) >> 4);
 #pragma unroll
-                    for (int k = 0; k < HD / 16; k++) {
-                        const uint32_t at = (uint32_t)((k >> 2) * (kPT * 128) + (k & 3) * 32);
-                        umma_f16(d, desc_k((h ? ql : qh) + at), desc_k(k0 + at), kIdescQK, (h | k) != 0);
+                        for (int k = 0; k < (HD < 64 ? HD / 16 : 4); k++) umma_f16(d, a + 2 * k, b + 2 * k, kIdescQK, (h | c | k) != 0);
                     }
                 umma_commit(kEmpty(j & 1));
                 umma_commit(sFull(j % 3));
-                return true;
             };
-            bool ok = mbar_wait(qReady, 0, &s_abort, p.error, 349) && scores(0);
-            for (int j = 0; j < tiles && ok; j++) {
-                if (j + 1 < tiles) ok = scores(j + 1);
-                if (!ok || !mbar_wait(vFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 347) || !mbar_wait(pReady(j % 3), (j / 3) & 1, &s_abort, p.error, 348)) break;
+            if (mbar_wait(qReady, 0, &s_abort, p.error, 349) && mbar_wait(firstKeys, 0, &s_abort, p.error, 346)) {
                 tc_fence_after();
-                const uint32_t v0 = base + (4 + (j & 1)) * S::kTile, a = tmem + (uint32_t)(j % 3 * kPT);
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int k = 0; k < kPT / 16; k++) umma_f16_ta(tmem + kO, a + (k >> 1) * 32 + h * 16 + (k & 1) * 8, desc_mn(v0 + k * 2048), kIdescPV, (j | h | k) != 0);
-                umma_commit(vEmpty(j & 1));
+                scores(0);
+#pragma unroll 1
+                for (int j = 0; j < tiles; j++) {
+                    // values of tile j: the keys of j + 1 were converted before them, and P·V of j - 2, which read the scores' buffer of j + 1, was
+                    // done before they came
+                    if (!mbar_wait(vFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 347)) break;
+                    tc_fence_after();
+                    if (j + 1 < tiles) scores(j + 1);
+                    if (!mbar_wait(pReady(j % 3), (j / 3) & 1, &s_abort, p.error, 348)) break;
+                    tc_fence_after();
+                    const uint64_t v0 = desc_mn(base + (4 + (j & 1)) * S::kTile);
+                    const uint32_t a = tmem + (uint32_t)(j % 3 * kPT);
+#pragma unroll 2
+                    for (int k = 0; k < kPT / 16; k++) {
+                        umma_f16_ta(tmem + kO, a + (k >> 1) * 32 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, (j | k) != 0);
+                        umma_f16_ta(tmem + kO, a + (k >> 1) * 32 + 16 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, 1);
+                    }
+                    umma_commit(vEmpty(j & 1));
+                }
             }
         }
         __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 13) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+    if (warp == 17) { tc_fence_after(); tmem_dealloc(tmem, 512); }
 }
 
 // ───────────── weights of the last tokens ─────────────
@@ -423,6 +483,7 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
     __shared__ __align__(8) unsigned long long s_bar;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
+    __shared__ float s_factor[kPT];
     __shared__ float4 s_row[kPT];                 // factor, maximum, 1 / sum, newest key of every query row
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = blockIdx.y, b = blockIdx.z;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -450,16 +511,21 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
             const uint4* const from = reinterpret_cast<const uint4*>(p.cache + (((size_t)b * p.G + g) * p.pages + pg) * Q4Page<NB>::kBytes);
             for (int i = lane; i < Q4Page<NB>::kHalf / 16; i += 32) reinterpret_cast<uint4*>(half)[i] = from[i];
             __syncwarp();
-            convert_row<NB>(half, lane, smem + 2 * S::kTile, tid);
-        } else zero_row<NB>(smem + 2 * S::kTile, tid);
+            convert_row<NB>(half, lane, smem + 2 * S::kTile, tid, 0, 4);
+        } else zero_row<NB>(smem + 2 * S::kTile, tid, 0, 4);
         int phase = 0;
         for (int r0 = 0; r0 < rows; r0 += kPT) {
             const int r = r0 + tid, t = room - window + r / p.ratio, head = g * p.ratio + r % p.ratio, m = first + t;
             const bool on = r < rows;
-            const float c = query_row<NB>(p, m, head, pos + t, on, smem, smem + S::kTile, tid);
+            query_rows<NB>(p, warp, 4, lane, smem, smem + S::kTile, s_factor, [&](int i, int& qm, int& qh, int& qp) {
+                const int of = (r0 + i) / p.ratio, token = room - window + of;
+                qm = first + token; qh = g * p.ratio + r0 + i - of * p.ratio; qp = pos + token;
+                return r0 + i < rows;
+            });
+            __syncthreads();
             float2 st = make_float2(0.0f, 1.0f);
             if (on) st = *reinterpret_cast<const float2*>(p.stats + ((size_t)m * p.H + head) * 2);
-            s_row[tid] = make_float4(c, -st.x, 1.0f / st.y, __int_as_float(on ? len + t : -1));
+            s_row[tid] = make_float4(s_factor[tid], -st.x, 1.0f / st.y, __int_as_float(on ? len + t : -1));
             fence_proxy_async_smem();
             tc_fence_before();
             __syncthreads();
