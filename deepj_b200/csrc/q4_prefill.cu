@@ -1,16 +1,19 @@
 // Packed prompts over the 4-bit cache on the 5th-generation tensor cores.
 //
 // A block takes 128 query rows of one key/value head: 128 / R consecutive tokens of one sequence times the R query heads that share the head, so that a
-// key or value is brought and converted once for all of them.  It walks the cached rows in tiles of 128:
+// key or value is brought and converted once for all of them.  It walks the cached rows in tiles of 64:
 //   S = Q·Kᵀ    Q in fp16 halves hi + lo of the rotated row times a power of two (22 bits); a stored key, code · scale, is exact in fp16: two MMAs
 //   P = 2^(S·c − m) per row, in halves hi + lo again, written over S in tensor memory, from where it is the A operand of
 //   O += P·V    with O in tensor memory as well
-//   warps 0-7   two threads to a row: running maximum and sum of the softmax in fp32, no exchange between lanes.  O is multiplied by the change of the
+//   warps 0-3   a thread is a row: running maximum and sum of the softmax in fp32, no exchange between lanes.  O is multiplied by the change of the
 //               maximum only when that grew by more than 2^8: until then P is larger than one, which fp16 and the fp32 sums have room for
-//   warps 8-15  two warps are a page: 4-bit codes → fp16 tiles with 128-byte swizzle, keys a tile ahead of the values
-//   warp 16     one thread brings the pages' halves with bulk copies into a ring
-//   warp 17     one thread issues the MMAs: Q·K of the next tile before P·V of this one, so that the softmax never waits for them
-// Tensor memory: three S/P buffers of 128 columns and O.  Every wait is bounded (codes 341-349 in the device error word).
+//   warps 4-11  four for keys, four for values, sixteen rows of a tile each: bulk copies into a place of their own, the codes into registers, and when the
+//               tile is free 4-bit codes → fp16 with 128-byte swizzle
+//   warp 12     issues the MMAs: Q·K of the next tile before P·V of this one
+// The chain from scores over weights to values leaves every unit idle most of the time, and a satisfied wait on a barrier costs 170 cycles: two blocks
+// share an SM (half of its tensor and shared memory each: two S/P buffers of 64 columns, O, one tile of keys and one of values).  One block per SM with
+// tiles of 128 keys and two of each took 3900 cycles for 128 keys, where the MMAs take 2048.
+// Every wait is bounded (codes 341-350 in the device error word).
 #include <algorithm>
 #include <cmath>
 
@@ -22,9 +25,9 @@
 namespace dj {
 namespace {
 
-constexpr int kPT = 128;                          // query rows and keys of a tile
-constexpr int kPThreads = 576;                    // warps: 8 softmax, 8 conversion, copies, MMAs
-constexpr int kPRing = 3;                         // ring stages: the K or the V halves of a tile's four pages
+constexpr int kPT = 128;                          // query rows of a tile
+constexpr int kKT = 64;                           // keys of a tile: two pages
+constexpr int kPThreads = 416;                    // warps: 4 softmax, 8 conversion, MMAs
 
 struct PrefillParams {
     const float* qkv; int q_off, ld;
@@ -37,20 +40,20 @@ struct PrefillParams {
 };
 
 template <int NB> struct PrefillShape {
-    static constexpr int HD = 32 * NB, kChunks = (HD + 63) / 64, kTile = kChunks * kPT * 128;      // bytes of 128 rows in 128-byte pieces
-    static constexpr int kStage = 4 * Q4Page<NB>::kHalf;
-    static constexpr int kRingAt = 6 * kTile;                            // Q hi, Q lo, K × 2, V × 2
-    static constexpr size_t kUsed = (size_t)kRingAt + kPRing * kStage + 1024;
-    static constexpr size_t kSmem = kUsed > 120 * 1024 ? kUsed : 120 * 1024;      // one block per SM: it holds all tensor memory
+    static constexpr int HD = 32 * NB, kChunks = (HD + 63) / 64;         // 128-byte pieces of a row
+    static constexpr int kQ = kChunks * kPT * 128, kKV = kChunks * kKT * 128;      // bytes of a tile of queries (hi or lo), of keys or values
+    static constexpr int kKAt = 2 * kQ, kVAt = kKAt + kKV, kRawAt = kVAt + kKV, kRaw = 16 * (Q4Page<NB>::kRow + 2 * NB);      // kRaw: sixteen rows' codes and scales
+    static constexpr size_t kUsed = (size_t)kRawAt + 8 * kRaw + 1024;
+    static constexpr size_t kSmem = kUsed > 80 * 1024 ? kUsed : 80 * 1024;         // two blocks per SM: they hold all tensor memory
 };
 
 // K-major, 128-byte swizzle: 8-row groups 1024 bytes apart
 __device__ __forceinline__ uint64_t desc_k(uint32_t a) {
     return (uint64_t)((a >> 4) & 0x3fff) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// MN-major: 64 dims to a 128-byte row, 8-key groups 1024 bytes apart, the next 64 dims 128 rows on
+// MN-major: 64 dims to a 128-byte row, 8-key groups 1024 bytes apart, the next 64 dims kKT rows on
 __device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3fff) | ((uint64_t)(kPT * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+    return (uint64_t)((a >> 4) & 0x3fff) | ((uint64_t)(kKT * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
@@ -80,7 +83,7 @@ __device__ __forceinline__ uint32_t half_of(uint32_t moved, __half2 scale, __hal
     const __half2 r = wide ? __hmul2(__hsub2(v, __float2half2_rn(24.0f)), scale) : __hfma2(v, scale, off);
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-template <int NB, bool WIDE>
+template <int NB, int ROWS, bool WIDE>
 __device__ __forceinline__ void convert_words(const unsigned char* half, int lane, unsigned char* tile, int row, const __half2 (&scale)[NB], int t0, int t1) {
     __half2 off[NB];
 #pragma unroll
@@ -92,14 +95,35 @@ __device__ __forceinline__ void convert_words(const unsigned char* half, int lan
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             const int c = 4 * j + t;
-            *reinterpret_cast<uint4*>(tile + (j >> 1) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(tile + (j >> 1) * (ROWS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
                 make_uint4(half_of(w[j] << 6, scale[j], off[j], WIDE), half_of(w[j] << 2, scale[j], off[j], WIDE), half_of(w[j] >> 2, scale[j], off[j], WIDE),
                            half_of(w[j] >> 6, scale[j], off[j], WIDE));
         }
     }
 }
-// Row `lane` of a page's K or V half, its words (t0 … t1 - 1, j) → row `row` of an fp16 tile.
-template <int NB>
+// Pieces t0, t0 + 1 of a row, in registers, → row `row` of an fp16 tile of ROWS rows.
+template <int NB, int ROWS>
+__device__ __forceinline__ void convert_pieces(const uint32_t (&w)[2][NB], const float (&s)[NB], unsigned char* tile, int row, int t0) {
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NB; j++) most = fmaxf(most, s[j]);
+    auto all = [&](bool wide) {
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const __half2 scale = __float2half2_rn(s[j]), off = __hmul2(scale, __float2half2_rn(-24.0f));
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int c = 4 * j + t0 + u;
+                *reinterpret_cast<uint4*>(tile + (j >> 1) * (ROWS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                    make_uint4(half_of(w[u][j] << 6, scale, off, wide), half_of(w[u][j] << 2, scale, off, wide), half_of(w[u][j] >> 2, scale, off, wide),
+                               half_of(w[u][j] >> 6, scale, off, wide));
+            }
+        }
+    };
+    if (__any_sync(0xffffffffu, most > 2048.0f)) all(true); else all(false);
+}
+// Row `lane` of a page's K or V half, its words (t0 … t1 - 1, j) → row `row` of an fp16 tile of ROWS rows.
+template <int NB, int ROWS>
 __device__ __forceinline__ void convert_row(const unsigned char* half, int lane, unsigned char* tile, int row, int t0, int t1) {
     __half2 scale[NB];
     float most = 0.0f;
@@ -109,14 +133,14 @@ __device__ __forceinline__ void convert_row(const unsigned char* half, int lane,
         most = fmaxf(most, s);
         scale[j] = __float2half2_rn(s);
     }
-    if (__any_sync(0xffffffffu, most > 2048.0f)) convert_words<NB, true>(half, lane, tile, row, scale, t0, t1);
-    else convert_words<NB, false>(half, lane, tile, row, scale, t0, t1);
+    if (__any_sync(0xffffffffu, most > 2048.0f)) convert_words<NB, ROWS, true>(half, lane, tile, row, scale, t0, t1);
+    else convert_words<NB, ROWS, false>(half, lane, tile, row, scale, t0, t1);
 }
-template <int NB>
+template <int NB, int ROWS>
 __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, int t1) {
 #pragma unroll 1
     for (int c = 0; c < 4 * NB; c++)
-        if ((c & 3) >= t0 && (c & 3) < t1) *reinterpret_cast<uint4*>(tile + (c >> 3) * (kPT * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        if ((c & 3) >= t0 && (c & 3) < t1) *reinterpret_cast<uint4*>(tile + (c >> 3) * (ROWS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
 }
 
 // Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 8·NB lanes of four values each; `place(row, m, head, position)` says
@@ -198,39 +222,34 @@ __device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int to
 }
 
 template <int NB>
-__global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams p) {
+__global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams p) {
     using S = PrefillShape<NB>;
     constexpr int HD = S::HD;
-    constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kPT >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);      // fp16 × fp16 → fp32
+    constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kKT >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);      // fp16 × fp16 → fp32
     constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);      // B MN-major
-    constexpr uint32_t kO = 3 * kPT;              // O's first column
+    constexpr uint32_t kO = 2 * kKT;              // O's first column
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long s_bar[2 * kPRing + 14];
+    __shared__ __align__(8) unsigned long long s_bar[8 + 9];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
-    __shared__ float s_max[2][2][kPT], s_factor[kPT];
+    __shared__ float s_factor[kPT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
     auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
-    auto ringFull = [&](int s) { return bar(s); };
-    auto ringEmpty = [&](int s) { return bar(kPRing + s); };
-    auto kEmpty = [&](int s) { return bar(2 * kPRing + s); };           // Q·K of a tile is done
-    auto vFull = [&](int s) { return bar(2 * kPRing + 2 + s); };         // the values of a tile stand, and so do the keys of the next one
-    auto vEmpty = [&](int s) { return bar(2 * kPRing + 4 + s); };        // P·V of a tile is done
-    auto sFull = [&](int s) { return bar(2 * kPRing + 6 + s); };
-    auto pReady = [&](int s) { return bar(2 * kPRing + 9 + s); };
-    const uint32_t qReady = bar(2 * kPRing + 12), firstKeys = bar(2 * kPRing + 13);
+    const uint32_t kFull = bar(8), kEmpty = bar(9), vFull = bar(10), vEmpty = bar(11);      // one phase a tile; bars 0-7: the conversion warps' copies
+    auto sFull = [&](int s) { return bar(12 + s); };
+    auto pReady = [&](int s) { return bar(14 + s); };
+    const uint32_t qReady = bar(16);
     if (tid == 0) {
-        for (int s = 0; s < kPRing; s++) { mbar_init(ringFull(s), 1); mbar_init(ringEmpty(s), 8); }
-        for (int s = 0; s < 2; s++) { mbar_init(kEmpty(s), 1); mbar_init(vFull(s), 8); mbar_init(vEmpty(s), 1); }
-        for (int s = 0; s < 3; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 8); }
-        mbar_init(qReady, 8);
-        mbar_init(firstKeys, 8);
+        for (int s = 0; s < 8; s++) mbar_init(bar(s), 1);
+        mbar_init(kFull, 4); mbar_init(kEmpty, 1); mbar_init(vFull, 4); mbar_init(vEmpty, 1);
+        for (int s = 0; s < 2; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 4); }
+        mbar_init(qReady, 4);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 17) tmem_alloc(smem_u32(&s_tmem), 512);
+    if (warp == 12) tmem_alloc(smem_u32(&s_tmem), 256);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -245,18 +264,16 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
         room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
     }
     const int used = max(0, min(tokensPerTile, room - t0));              // tokens of this tile
-    const int keys = used > 0 ? len + t0 + used : 0, tiles = (keys + kPT - 1) / kPT, pages = (keys + kQ4Page - 1) / kQ4Page;
+    const int keys = used > 0 ? len + t0 + used : 0, tiles = (keys + kKT - 1) / kKT, pages = (keys + kQ4Page - 1) / kQ4Page;
 
-    if (warp < 8) {
-        // two threads to a row, 64 keys of a tile each: warps w and w + 4 exchange what they find through shared memory
-        const int part = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, token = row / p.ratio, head = g * p.ratio + row % p.ratio;
+    if (warp < 4) {
+        const int row = tid, token = row / p.ratio, head = g * p.ratio + row % p.ratio;
         const bool on = token < used;
         const int m = first + t0 + token, last = on ? len + t0 + token : -1;      // the row's place in the buffers, its newest key
-        auto meet = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
         float c = 1.0f, top = -INFINITY;
         float2 sums = make_float2(0.0f, 0.0f);
         if (tiles > 0) {
-            query_rows<NB>(p, warp, 8, lane, smem, smem + S::kTile, s_factor, [&](int r, int& qm, int& qh, int& qp) {
+            query_rows<NB>(p, warp, 4, lane, smem, smem + S::kQ, s_factor, [&](int r, int& qm, int& qh, int& qp) {
                 const int t = r / p.ratio;
                 qm = first + t0 + t; qh = g * p.ratio + r - t * p.ratio; qp = pos + t0 + t;
                 return t < used;
@@ -264,17 +281,18 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(qReady);
-            asm volatile("bar.sync 5, 256;" ::: "memory");
+            asm volatile("bar.sync 1, 128;" ::: "memory");
             c = s_factor[row];
         }
-        const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
         bool ok = true;
+#pragma unroll 1
         for (int j = 0; j < tiles; j++) {
-            if (!__all_sync(0xffffffffu, mbar_wait(sFull(j % 3), (j / 3) & 1, &s_abort, p.error, 341))) ok = false;
+            if (!__all_sync(0xffffffffu, mbar_wait(sFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 341))) ok = false;
             tc_fence_after();
-            const uint32_t at = mine + (uint32_t)(j % 3 * kPT + part * 64);
-            const int left = last - j * kPT - part * 64;                 // newest key within these 64
-            const bool cut = !__all_sync(0xffffffffu, left >= 63);
+            const uint32_t at = mine + (uint32_t)((j & 1) * kKT);
+            const int left = last - j * kKT;                             // newest key within the tile
+            const bool cut = !__all_sync(0xffffffffu, left >= kKT - 1);
             float most = -INFINITY;
             // columns are read twice, 32 a time, rather than kept: less code and registers for a load that takes 50 cycles
             auto columns = [&](int q, uint32_t (&v)[32]) {
@@ -285,7 +303,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
                         if (k > left - q * 32) v[k] = 0xff800000u;
             };
 #pragma unroll 1
-            for (int q = 0; q < 2; q++) {
+            for (int q = 0; q < kKT / 32; q++) {
                 uint32_t v[32];
                 columns(q, v);
                 float m2[2] = {most, -INFINITY};
@@ -294,17 +312,14 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
                 most = fmaxf(m2[0], m2[1]);
             }
             most *= c;
-            s_max[j & 1][part][row] = most;
-            meet();
-            most = fmaxf(most, s_max[j & 1][1 - part][row]);
             const bool grown = most > top + 8.0f;                        // also the first keys of a row
-            if (__any_sync(0xffffffffu, grown)) {                        // both warps of a row come to the same
+            if (__any_sync(0xffffffffu, grown)) {
                 const float now = grown ? most : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
                 if (j > 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(vEmpty((j - 1) & 1), ((j - 1) >> 1) & 1, &s_abort, p.error, 342))) ok = false;
+                    if (!__all_sync(0xffffffffu, mbar_wait(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int k = 32 * part; k < HD; k += 64) {
+                    for (int k = 0; k < HD; k += 32) {
                         uint32_t o[32];
                         tmem_ld32(mine + kO + k, o);
 #pragma unroll
@@ -318,7 +333,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
             const float shift = top > -INFINITY ? -top : 0.0f;           // a row without keys yet: every weight is 2^-inf
             const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift), minus = make_float2(-1.0f, -1.0f);
 #pragma unroll 1
-            for (int q = 0; q < 2; q++) {
+            for (int q = 0; q < kKT / 32; q++) {
                 uint32_t v[32], w[32];
                 columns(q, v);
 #pragma unroll
@@ -337,23 +352,17 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(pReady(j % 3));
-        }
-        float sum = sums.x + sums.y;
-        if (tiles > 0) {
-            s_max[tiles & 1][part][row] = sum;
-            meet();
-            sum += s_max[tiles & 1][1 - part][row];
+            if (lane == 0) mbar_arrive(pReady(j & 1));
         }
         if (tiles > 0) {
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(vEmpty((tiles - 1) & 1), ((tiles - 1) >> 1) & 1, &s_abort, p.error, 343));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(vEmpty, (tiles - 1) & 1, &s_abort, p.error, 343));
             tc_fence_after();
-            const float inv = 1.0f / sum;
+            const float sum = sums.x + sums.y, inv = 1.0f / sum;
             constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;
             float* const stage = reinterpret_cast<float*>(smem);
 #pragma unroll 1
-            for (int k = 32 * part; ok && k < HD; k += 64) {
+            for (int k = 0; ok && k < HD; k += 32) {
                 uint32_t o[32];
                 tmem_ld32(mine + kO + k, o);
 #pragma unroll
@@ -363,106 +372,103 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
                         make_float4(__uint_as_float(o[from]) * inv, __uint_as_float(o[from + 4]) * inv, __uint_as_float(o[from + 1]) * inv, __uint_as_float(o[from + 5]) * inv);
                 }
             }
-            asm volatile("bar.sync 5, 256;" ::: "memory");
-            for (int r = warp * RPW + lane / LPR; ok && r < used * p.ratio; r += 8 * RPW) {
-                const int t = r / p.ratio, e = lane % LPR;
-                *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) =
-                    *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
+            __syncwarp();                         // a warp stores the rows that it has staged
+#pragma unroll 4
+            for (int i = lane / LPR; ok && i < 32; i += RPW) {
+                const int r = warp * 32 + i, t = r / p.ratio, e = lane % LPR;
+                if (t < used)
+                    *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) =
+                        *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
             }
-            if (part == 0 && on && p.stats != nullptr && t0 + token >= room - p.window)
+            if (on && p.stats != nullptr && t0 + token >= room - p.window)
                 *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
         }
-    } else if (warp < 16) {
-        const int w = warp & 3, t0 = (warp - 8) >> 2 << 1;               // page of the tile, half of a row's words
-        bool ok = true;
-        int item = 0;
+    } else if (warp < 12) {
+        const bool value = warp >= 8;
+        const int w = warp & 3, row = 16 * w + (lane & 15), t0w = lane >> 4 << 1;        // row of the tile, first of this lane's two pieces
+        unsigned char* const raw_at = smem + S::kRawAt + (warp - 4) * S::kRaw;
+        unsigned char* const tile = smem + (value ? S::kVAt : S::kKAt);
+        const uint32_t arrived = bar(warp - 4);
+        const unsigned char* from = p.cache + (((size_t)b * p.G + g) * p.pages + (w >> 1)) * Q4Page<NB>::kBytes + (value ? Q4Page<NB>::kV : 0);
+        auto request = [&](int j) {               // this warp's rows of tile j
+            if (lane == 0 && j < tiles && 2 * j + (w >> 1) < pages) {
+                const unsigned char* const page = from + (size_t)(2 * j) * Q4Page<NB>::kBytes;
+                mbar_arrive_expect_tx(arrived, S::kRaw);
+                bulk_g2s(smem_u32(raw_at), page + (w & 1) * (16 * Q4Page<NB>::kRow), 16 * Q4Page<NB>::kRow, arrived);
+                bulk_g2s(smem_u32(raw_at) + 16 * Q4Page<NB>::kRow, page + Q4Page<NB>::kKs + (w & 1) * (32 * NB), 32 * NB, arrived);
+            }
+        };
+        request(0);
 #pragma unroll 1
-        for (int i = 0; i < 2 * tiles && ok; i++) {                      // K 0, K 1, V 0, K 2, V 1, …, V tiles - 1
-            const bool value = i > 0 && (i % 2 == 0 || i == 2 * tiles - 1);
-            const int j = i == 0 ? 0 : value ? (i - 1) / 2 : (i + 1) / 2;
-            if (j >= 2 && !__all_sync(0xffffffffu, mbar_wait(value ? vEmpty(j & 1) : kEmpty(j & 1), ((j >> 1) - 1) & 1, &s_abort, p.error, 344))) break;
-            if (!__all_sync(0xffffffffu, mbar_wait(ringFull(item % kPRing), (item / kPRing) & 1, &s_abort, p.error, 345))) break;
-            unsigned char* const tile = smem + (value ? 4 + (j & 1) : 2 + (j & 1)) * S::kTile;
-            if (4 * j + w < pages) convert_row<NB>(smem + S::kRingAt + item % kPRing * S::kStage + w * Q4Page<NB>::kHalf, lane, tile, 32 * w + lane, t0, t0 + 2);
-            else if (value) zero_row<NB>(tile, 32 * w + lane, t0, t0 + 2);      // weights of 0 meet no garbage
+        for (int j = 0; j < tiles; j++) {
+            const bool there = 2 * j + (w >> 1) < pages;
+            uint32_t words[2][NB];
+            float scale[NB];
+            if (there) {
+                if (!__all_sync(0xffffffffu, mbar_wait(arrived, j & 1, &s_abort, p.error, 345))) break;
+                piece_of<NB>(words[0], raw_at + Q4Page<NB>::word(lane & 15, t0w, 0));
+                piece_of<NB>(words[1], raw_at + Q4Page<NB>::word(lane & 15, t0w + 1, 0));
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+                    scale[i] = __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(raw_at + 16 * Q4Page<NB>::kRow + ((lane & 15) * NB + i) * 2) << 16);
+                __syncwarp();
+                request(j + 1);                   // everything of this tile is in registers
+            }
+            if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait(value ? vEmpty : kEmpty, (j - 1) & 1, &s_abort, p.error, 344))) break;
+            if (there) convert_pieces<NB, kKT>(words, scale, tile, row, t0w);
+            else if (value) zero_row<NB, kKT>(tile, row, t0w, t0w + 2);      // weights of 0 meet no garbage
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(ringEmpty(item % kPRing));
-                if (value) mbar_arrive(vFull(j & 1));
-                else if (j == 0) mbar_arrive(firstKeys);
-            }
-            item++;
+            if (lane == 0) mbar_arrive(value ? vFull : kFull);
         }
-    } else if (warp == 16) {
-        if (lane == 0) {
-            const unsigned char* const plane = p.cache + ((size_t)b * p.G + g) * p.pages * Q4Page<NB>::kBytes;
-            int item = 0;
-            bool ok = true;
-            auto bring = [&](int j, bool value) {
-                const int s = item % kPRing, n = min(4, pages - 4 * j);
-                if (item >= kPRing && !mbar_wait(ringEmpty(s), (item / kPRing - 1) & 1, &s_abort, p.error, 346)) return false;
-                mbar_arrive_expect_tx(ringFull(s), n * Q4Page<NB>::kHalf);
-                for (int w = 0; w < n; w++)
-                    bulk_g2s(base + S::kRingAt + s * S::kStage + w * Q4Page<NB>::kHalf, plane + (size_t)(4 * j + w) * Q4Page<NB>::kBytes + (value ? Q4Page<NB>::kV : 0),
-                             Q4Page<NB>::kHalf, ringFull(s));
-                item++;
-                return true;
-            };
-            for (int j = 0; j <= tiles && ok; j++) {
-                if (j < tiles) ok = bring(j, false);
-                if (ok && j > 0) ok = bring(j - 1, true);
-            }
-            if (!ok)                              // a wait ran out: let the copies in flight land before the block goes
-                for (int back = 1; back <= kPRing && back <= item; back++)
-                    for (unsigned n = 0; n < (1u << 16) && !mbar_try_wait(ringFull((item - back) % kPRing), ((item - back) / kPRing) & 1); n++) {}
-        }
-        __syncwarp();
     } else {
-        if (lane == 0 && tiles > 0) {
-            // rolled: what one thread issues has to come from the instruction cache in time
-            auto scores = [&](int j) {
-                const uint32_t d = tmem + (uint32_t)(j % 3 * kPT);
-                const uint64_t q0 = desc_k(base), k0 = desc_k(base + (2 + (j & 1)) * S::kTile);
-#pragma unroll 1
-                for (int h = 0; h < 2; h++)
-#pragma unroll 1
-                    for (int c = 0; c < S::kChunks; c++) {
-                        const uint64_t a = q0 + (uint32_t)((h * S::kTile + c * (kPT * 128)) >> 4), b = k0 + (uint32_t)((c * (kPT * 128)) >> 4);
+        // The whole warp walks the loop and one lane's predicate issues: in one lane's branch every operand would be moved into a uniform register first (70
+        // cycles an MMA).  Rolled: what is issued has to come from the instruction cache in time.
+        const uint32_t lead = elect_one();
+        auto waited = [&](uint32_t on, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(on, parity, &s_abort, p.error, code)); };
+        auto scores = [&](int j) {
+            const uint32_t d = tmem + (uint32_t)((j & 1) * kKT);
+            const uint64_t q0 = desc_k(base), k0 = desc_k(base + S::kKAt);
 #pragma unroll
-                        for (int k = 0; k < (HD < 64 ? HD / 16 : 4); k++) umma_f16(d, a + 2 * k, b + 2 * k, kIdescQK, (h | c | k) != 0);
-                    }
-                umma_commit(kEmpty(j & 1));
-                umma_commit(sFull(j % 3));
-            };
-            if (mbar_wait(qReady, 0, &s_abort, p.error, 349) && mbar_wait(firstKeys, 0, &s_abort, p.error, 346)) {
-                tc_fence_after();
-                scores(0);
-#pragma unroll 1
-                for (int j = 0; j < tiles; j++) {
-                    // values of tile j: the keys of j + 1 were converted before them, and P·V of j - 2, which read the scores' buffer of j + 1, was
-                    // done before they came
-                    if (!mbar_wait(vFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 347)) break;
-                    tc_fence_after();
-                    if (j + 1 < tiles) scores(j + 1);
-                    if (!mbar_wait(pReady(j % 3), (j / 3) & 1, &s_abort, p.error, 348)) break;
-                    tc_fence_after();
-                    const uint64_t v0 = desc_mn(base + (4 + (j & 1)) * S::kTile);
-                    const uint32_t a = tmem + (uint32_t)(j % 3 * kPT);
-#pragma unroll 2
-                    for (int k = 0; k < kPT / 16; k++) {
-                        umma_f16_ta(tmem + kO, a + (k >> 1) * 32 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, (j | k) != 0);
-                        umma_f16_ta(tmem + kO, a + (k >> 1) * 32 + 16 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, 1);
-                    }
-                    umma_commit(vEmpty(j & 1));
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int c = 0; c < S::kChunks; c++) {
+                    const uint64_t a = q0 + (uint32_t)((h * S::kQ + c * (kPT * 128)) >> 4), b = k0 + (uint32_t)((c * (kKT * 128)) >> 4);
+#pragma unroll
+                    for (int k = 0; k < (HD < 64 ? HD / 16 : 4); k++) umma_f16_by(lead, d, a + 2 * k, b + 2 * k, kIdescQK, (h | c | k) != 0);
                 }
+            umma_commit_by(lead, kEmpty);
+            umma_commit_by(lead, sFull(j & 1));
+        };
+        if (tiles > 0 && waited(qReady, 0, 349) && waited(kFull, 0, 346)) {
+            tc_fence_after();
+            scores(0);
+#pragma unroll 1
+            for (int j = 0; j < tiles; j++) {
+                if (j + 1 < tiles) {
+                    // P·V of tile j - 1 has read the buffer that the scores of j + 1 go to
+                    if (j >= 1 && !waited(vEmpty, (j - 1) & 1, 350)) break;
+                    if (!waited(kFull, (j + 1) & 1, 347)) break;
+                    tc_fence_after();
+                    scores(j + 1);
+                }
+                if (!waited(vFull, j & 1, 347) || !waited(pReady(j & 1), (j >> 1) & 1, 348)) break;
+                tc_fence_after();
+                const uint64_t v0 = desc_mn(base + S::kVAt);
+                const uint32_t a = tmem + (uint32_t)((j & 1) * kKT);
+#pragma unroll
+                for (int k = 0; k < kKT / 16; k++) {
+                    umma_f16_ta_by(lead, tmem + kO, a + (k >> 1) * 32 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, (j | k) != 0);
+                    umma_f16_ta_by(lead, tmem + kO, a + (k >> 1) * 32 + 16 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, 1);
+                }
+                umma_commit_by(lead, vEmpty);
             }
         }
         __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 17) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+    if (warp == 12) { tc_fence_after(); tmem_dealloc(tmem, 256); }
 }
 
 // ───────────── weights of the last tokens ─────────────
@@ -470,7 +476,7 @@ __global__ void __launch_bounds__(kPThreads, 1) k_q4_prefill(const PrefillParams
 // Sᵀ = K·Qᵀ, so that a thread is a key and adds up its row over the queries in a fixed order.  A block takes 128 keys and 128 query rows at a time.
 constexpr int kWThreads = 128;
 template <int NB> struct WindowShape {
-    static constexpr int kTile = PrefillShape<NB>::kTile;
+    static constexpr int kTile = PrefillShape<NB>::kQ;
     static constexpr int kHalvesAt = 3 * kTile;                          // Q hi, Q lo, K
     static constexpr size_t kSmem = (size_t)kHalvesAt + 4 * Q4Page<NB>::kHalf + 1024;
 };
@@ -511,8 +517,8 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
             const uint4* const from = reinterpret_cast<const uint4*>(p.cache + (((size_t)b * p.G + g) * p.pages + pg) * Q4Page<NB>::kBytes);
             for (int i = lane; i < Q4Page<NB>::kHalf / 16; i += 32) reinterpret_cast<uint4*>(half)[i] = from[i];
             __syncwarp();
-            convert_row<NB>(half, lane, smem + 2 * S::kTile, tid, 0, 4);
-        } else zero_row<NB>(smem + 2 * S::kTile, tid, 0, 4);
+            convert_row<NB, kPT>(half, lane, smem + 2 * S::kTile, tid, 0, 4);
+        } else zero_row<NB, kPT>(smem + 2 * S::kTile, tid, 0, 4);
         int phase = 0;
         for (int r0 = 0; r0 < rows; r0 += kPT) {
             const int r = r0 + tid, t = room - window + r / p.ratio, head = g * p.ratio + r % p.ratio, m = first + t;
