@@ -39,6 +39,7 @@ struct PrefillParams {
     int* error;
 };
 
+constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
 template <int NB> struct PrefillShape {
     static constexpr int HD = 32 * NB, kChunks = (HD + 63) / 64;         // 128-byte pieces of a row
     static constexpr int kQ = kChunks * kPT * 128, kKV = kChunks * kKT * 128;      // bytes of a tile of queries (hi or lo), of keys or values
@@ -195,13 +196,14 @@ __device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
-// Sequence and first token of query tile `tile`, the last tile of a sequence first; whole warps call it.
-__device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int tokensPerTile, int lane, int& b, int& first, int& tokens, int& t0) {
+// Sequence, its place and the first token of query tile `tile`, the last tile of a sequence first; whole warps call it.
+__device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int tokensPerTile, int lane, int& b, int& first, int& tokens, int& t0, int& len, int& pos) {
     for (int b0 = 0; b0 < p.B; b0 += 32) {
-        int from = 0, n = 0;
+        int from = 0, n = 0, l = 0, q = 0;
         if (b0 + lane < p.B) {
             from = max(0, (int)p.starts[b0 + lane]);
             n = max(0, min(p.M, (int)p.starts[b0 + lane + 1]) - from);
+            l = (int)p.len[b0 + lane]; q = (int)p.pos[b0 + lane];
         }
         const int tiles = (n + tokensPerTile - 1) / tokensPerTile;
         int upto = tiles;
@@ -209,11 +211,12 @@ __device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int to
         for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
         const unsigned hit = __ballot_sync(0xffffffffu, tile < upto);
         if (hit) {
-            const int l = __ffs(hit) - 1;
-            b = b0 + l;
-            first = __shfl_sync(0xffffffffu, from, l);
-            tokens = __shfl_sync(0xffffffffu, n, l);
-            t0 = (__shfl_sync(0xffffffffu, upto, l) - 1 - tile) * tokensPerTile;
+            const int k = __ffs(hit) - 1;
+            b = b0 + k;
+            first = __shfl_sync(0xffffffffu, from, k);
+            tokens = __shfl_sync(0xffffffffu, n, k);
+            len = __shfl_sync(0xffffffffu, l, k); pos = __shfl_sync(0xffffffffu, q, k);
+            t0 = (__shfl_sync(0xffffffffu, upto, k) - 1 - tile) * tokensPerTile;
             return true;
         }
         tile -= __shfl_sync(0xffffffffu, upto, 31);
@@ -245,7 +248,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         for (int s = 0; s < 8; s++) mbar_init(bar(s), 1);
         mbar_init(kFull, 4); mbar_init(kEmpty, 1); mbar_init(vFull, 4); mbar_init(vEmpty, 1);
         for (int s = 0; s < 2; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 4); }
-        mbar_init(qReady, 4);
+        mbar_init(qReady, 12);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -259,13 +262,20 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
 
     const int g = blockIdx.x % p.G, tokensPerTile = kPT / p.ratio;
     int b = 0, first = 0, tokens = 0, t0 = 0, len = 0, pos = 0, room = 0;
-    if (tile_of(p, blockIdx.x / p.G, tokensPerTile, lane, b, first, tokens, t0)) {
-        len = (int)p.len[b]; pos = (int)p.pos[b];
-        room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
-    }
+    if (tile_of(p, blockIdx.x / p.G, tokensPerTile, lane, b, first, tokens, t0, len, pos)) room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
     const int used = max(0, min(tokensPerTile, room - t0));              // tokens of this tile
     const int keys = used > 0 ? len + t0 + used : 0, tiles = (keys + kKT - 1) / kKT, pages = (keys + kQ4Page - 1) / kQ4Page;
 
+    auto queries = [&]() {                        // twelve warps lay the queries down
+        query_rows<NB>(p, warp, 12, lane, smem, smem + S::kQ, s_factor, [&](int r, int& qm, int& qh, int& qp) {
+            const int t = r / p.ratio;
+            qm = first + t0 + t; qh = g * p.ratio + r - t * p.ratio; qp = pos + t0 + t;
+            return t < used;
+        });
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qReady);
+    };
     if (warp < 4) {
         const int row = tid, token = row / p.ratio, head = g * p.ratio + row % p.ratio;
         const bool on = token < used;
@@ -273,22 +283,16 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         float c = 1.0f, top = -INFINITY;
         float2 sums = make_float2(0.0f, 0.0f);
         if (tiles > 0) {
-            query_rows<NB>(p, warp, 4, lane, smem, smem + S::kQ, s_factor, [&](int r, int& qm, int& qh, int& qp) {
-                const int t = r / p.ratio;
-                qm = first + t0 + t; qh = g * p.ratio + r - t * p.ratio; qp = pos + t0 + t;
-                return t < used;
-            });
-            fence_proxy_async_smem();
+            queries();
+            mbar_wait_long(qReady, 0, &s_abort, p.error, 349);
             __syncwarp();
-            if (lane == 0) mbar_arrive(qReady);
-            asm volatile("bar.sync 1, 128;" ::: "memory");
             c = s_factor[row];
         }
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
         bool ok = true;
 #pragma unroll 1
         for (int j = 0; j < tiles; j++) {
-            if (!__all_sync(0xffffffffu, mbar_wait(sFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 341))) ok = false;
+            if (!__all_sync(0xffffffffu, mbar_wait_long(sFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 341))) ok = false;
             tc_fence_after();
             const uint32_t at = mine + (uint32_t)((j & 1) * kKT);
             const int left = last - j * kKT;                             // newest key within the tile
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             if (__any_sync(0xffffffffu, grown)) {
                 const float now = grown ? most : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
                 if (j > 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
+                    if (!__all_sync(0xffffffffu, mbar_wait_long(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
                     tc_fence_after();
 #pragma unroll 1
                     for (int k = 0; k < HD; k += 32) {
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         }
         if (tiles > 0) {
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
-            ok = __all_sync(0xffffffffu, ok && mbar_wait(vEmpty, (tiles - 1) & 1, &s_abort, p.error, 343));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_long(vEmpty, (tiles - 1) & 1, &s_abort, p.error, 343));
             tc_fence_after();
             const float sum = sums.x + sums.y, inv = 1.0f / sum;
             constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;
@@ -399,13 +403,14 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             }
         };
         request(0);
+        if (tiles > 0) queries();
 #pragma unroll 1
         for (int j = 0; j < tiles; j++) {
             const bool there = 2 * j + (w >> 1) < pages;
             uint32_t words[2][NB];
             float scale[NB];
             if (there) {
-                if (!__all_sync(0xffffffffu, mbar_wait(arrived, j & 1, &s_abort, p.error, 345))) break;
+                if (!__all_sync(0xffffffffu, mbar_wait_long(arrived, j & 1, &s_abort, p.error, 345))) break;
                 piece_of<NB>(words[0], raw_at + Q4Page<NB>::word(lane & 15, t0w, 0));
                 piece_of<NB>(words[1], raw_at + Q4Page<NB>::word(lane & 15, t0w + 1, 0));
 #pragma unroll
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 __syncwarp();
                 request(j + 1);                   // everything of this tile is in registers
             }
-            if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait(value ? vEmpty : kEmpty, (j - 1) & 1, &s_abort, p.error, 344))) break;
+            if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait_long(value ? vEmpty : kEmpty, (j - 1) & 1, &s_abort, p.error, 344))) break;
             if (there) convert_pieces<NB, kKT>(words, scale, tile, row, t0w);
             else if (value) zero_row<NB, kKT>(tile, row, t0w, t0w + 2);      // weights of 0 meet no garbage
             fence_proxy_async_smem();
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         // The whole warp walks the loop and one lane's predicate issues: in one lane's branch every operand would be moved into a uniform register first (70
         // cycles an MMA).  Rolled: what is issued has to come from the instruction cache in time.
         const uint32_t lead = elect_one();
-        auto waited = [&](uint32_t on, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(on, parity, &s_abort, p.error, code)); };
+        auto waited = [&](uint32_t on, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait_long(on, parity, &s_abort, p.error, code)); };
         auto scores = [&](int j) {
             const uint32_t d = tmem + (uint32_t)((j & 1) * kKT);
             const uint64_t q0 = desc_k(base), k0 = desc_k(base + S::kKAt);
@@ -501,87 +506,108 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
     }
     // before the next kernel may come in: its blocks could hold the tensor memory until this kernel is done
     if (warp == 0) tmem_alloc(smem_u32(&s_tmem), 128);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     pdl_wait();
     pdl_launch_dependents();
     const int first = max(0, (int)p.starts[b]), tokens = max(0, min(p.M, (int)p.starts[b + 1]) - first), len = (int)p.len[b], pos = (int)p.pos[b];
     const bool there = len >= 0 && len < p.maxSeq && pos >= 0 && pos < p.maxPos;
-    const int room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos), keys = there ? len + room : 0, k0 = blockIdx.x * kPT, key = k0 + tid;
-    const int window = min(p.window, room), rows = k0 < keys ? window * p.ratio : 0;
-    const size_t at = ((size_t)b * p.G + g) * p.maxSeq + key;
-    float add = 0.0f;
-    if (rows > 0) {
-        // the tile's keys: a warp is a page
-        const int pages = (keys + kQ4Page - 1) / kQ4Page, pg = k0 / kQ4Page + warp;
-        unsigned char* const half = smem + S::kHalvesAt + warp * Q4Page<NB>::kHalf;
-        if (pg < pages) {
-            const uint4* const from = reinterpret_cast<const uint4*>(p.cache + (((size_t)b * p.G + g) * p.pages + pg) * Q4Page<NB>::kBytes);
-            for (int i = lane; i < Q4Page<NB>::kHalf / 16; i += 32) reinterpret_cast<uint4*>(half)[i] = from[i];
+    const int room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos), keys = there ? len + room : 0, pages = (keys + kQ4Page - 1) / kQ4Page;
+    const int window = min(p.window, room), rows = window * p.ratio;
+    const uint32_t tmem = s_tmem;
+    unsigned char* const half = smem + S::kHalvesAt + warp * Q4Page<NB>::kHalf;
+    const unsigned char* const plane = p.cache + ((size_t)b * p.G + g) * p.pages * Q4Page<NB>::kBytes;
+    auto fetch = [&](int k0) {                    // this warp's page of a tile
+        const int pg = k0 / kQ4Page + warp;
+        if (k0 < keys && pg < pages)
+            for (int i = lane; i < Q4Page<NB>::kHalf / 16; i += 32) cp_async16(half + 16 * i, plane + (size_t)pg * Q4Page<NB>::kBytes + 16 * i);
+        cp_async_commit();
+    };
+    int phase = 0;
+    fetch((int)blockIdx.x * kPT);
+    for (int k0 = (int)blockIdx.x * kPT; k0 < keys; k0 += (int)gridDim.x * kPT) {
+        const int key = k0 + tid;
+        const size_t at = ((size_t)b * p.G + g) * p.maxSeq + key;
+        const float old = key < len ? p.acc[at] : 0.0f;
+        float add = 0.0f;
+        if (rows > 0) {
+            cp_async_wait<0>();
             __syncwarp();
-            convert_row<NB, kPT>(half, lane, smem + 2 * S::kTile, tid, 0, 4);
-        } else zero_row<NB, kPT>(smem + 2 * S::kTile, tid, 0, 4);
-        int phase = 0;
-        for (int r0 = 0; r0 < rows; r0 += kPT) {
-            const int r = r0 + tid, t = room - window + r / p.ratio, head = g * p.ratio + r % p.ratio, m = first + t;
-            const bool on = r < rows;
-            query_rows<NB>(p, warp, 4, lane, smem, smem + S::kTile, s_factor, [&](int i, int& qm, int& qh, int& qp) {
-                const int of = (r0 + i) / p.ratio, token = room - window + of;
-                qm = first + token; qh = g * p.ratio + r0 + i - of * p.ratio; qp = pos + token;
-                return r0 + i < rows;
-            });
-            __syncthreads();
-            float2 st = make_float2(0.0f, 1.0f);
-            if (on) st = *reinterpret_cast<const float2*>(p.stats + ((size_t)m * p.H + head) * 2);
-            s_row[tid] = make_float4(s_factor[tid], -st.x, 1.0f / st.y, __int_as_float(on ? len + t : -1));
-            fence_proxy_async_smem();
-            tc_fence_before();
-            __syncthreads();
-            tc_fence_after();
-            const uint32_t tmem = s_tmem;
-            if (tid == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int k = 0; k < HD / 16; k++) {
-                        const uint32_t o = (uint32_t)((k >> 2) * (kPT * 128) + (k & 3) * 32);
-                        umma_f16(tmem, desc_k(base + 2 * S::kTile + o), desc_k(base + h * S::kTile + o), kIdesc, (h | k) != 0);
-                    }
-                umma_commit(smem_u32(&s_bar));
-            }
+            if (k0 / kQ4Page + warp < pages) convert_row<NB, kPT>(half, lane, smem + 2 * S::kTile, tid, 0, 4);
+            else zero_row<NB, kPT>(smem + 2 * S::kTile, tid, 0, 4);
             __syncwarp();
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_bar), phase & 1, &s_abort, p.error, 350));
-            phase++;
-            tc_fence_after();
-#pragma unroll 1
-            for (int k = 0; ok && k < kPT && r0 + k < rows; k += 32) {
-                uint32_t v[32];
-                tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + k, v);
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    const float4 q = s_row[k + i];
-                    add += key <= __float_as_int(q.w) ? ex2(fmaf(__uint_as_float(v[i]), q.x, q.y)) * q.z : 0.0f;
+            fetch(k0 + (int)gridDim.x * kPT);
+            for (int r0 = 0; r0 < rows; r0 += kPT) {
+                const int n = min(rows - r0, kPT);
+                if (k0 == (int)blockIdx.x * kPT || rows > kPT) {         // the queries stay for all tiles if one tile holds them
+                    query_rows<NB>(p, warp, 4, lane, smem, smem + S::kTile, s_factor, [&](int i, int& qm, int& qh, int& qp) {
+                        const int of = (r0 + i) / p.ratio, token = room - window + of;
+                        qm = first + token; qh = g * p.ratio + r0 + i - of * p.ratio; qp = pos + token;
+                        return i < n;
+                    });
+                    __syncthreads();
+                    const int t = room - window + (r0 + tid) / p.ratio;
+                    float2 st = make_float2(0.0f, 1.0f);
+                    if (tid < n) st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(first + t) * p.H + g * p.ratio + (r0 + tid) % p.ratio) * 2);
+                    s_row[tid] = make_float4(s_factor[tid], -st.x, 1.0f / st.y, __int_as_float(tid < n ? len + t : -1));
                 }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncthreads();
+                tc_fence_after();
+                if (tid == 0) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++) {
+                            const uint32_t o = (uint32_t)((k >> 2) * (kPT * 128) + (k & 3) * 32);
+                            umma_f16(tmem, desc_k(base + 2 * S::kTile + o), desc_k(base + h * S::kTile + o), kIdesc, (h | k) != 0);
+                        }
+                    umma_commit(smem_u32(&s_bar));
+                }
+                __syncwarp();
+                const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_bar), phase & 1, &s_abort, p.error, 350));
+                phase++;
+                tc_fence_after();
+#pragma unroll 1
+                for (int k = 0; ok && k < n; k += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + k, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const float4 q = s_row[k + i];
+                        add += key <= __float_as_int(q.w) ? ex2(fmaf(__uint_as_float(v[i]), q.x, q.y)) * q.z : 0.0f;
+                    }
+                }
+                tc_fence_before();
+                __syncthreads();                  // the queries and the sums are read out
             }
-            tc_fence_before();
-            __syncthreads();                      // the queries and the sums are read out
         }
+        if (key < keys) p.accOut[at] = old + add;
     }
-    if (key < keys) p.accOut[at] = (key < len ? p.acc[at] : 0.0f) + add;
+    cp_async_wait<0>();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) { tc_fence_after(); tmem_dealloc(s_tmem, 128); }
+    if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem, 128); }
 }
 
 template <int NB>
 void prefill(const PrefillParams& p, cudaStream_t s) {
     static bool attr = false;
     if (!attr) {
-        DJ_CUDA_CHECK(cudaFuncSetAttribute(k_q4_prefill<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PrefillShape<NB>::kSmem));
+        DJ_CUDA_CHECK(cudaFuncSetAttribute(k_q4_prefill<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAlone));
         DJ_CUDA_CHECK(cudaFuncSetAttribute(k_q4_window<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WindowShape<NB>::kSmem));
         attr = true;
     }
     const int per = kPT / p.ratio;                // tokens of a tile; a sequence has at most one that is not full
-    if (p.M > 0) launch_k(k_q4_prefill<NB>, dim3(p.G * ((p.M + per - 1) / per + std::min(p.B, p.M) - 1)), dim3(kPThreads), PrefillShape<NB>::kSmem, s, true, p);
-    if (p.accOut != nullptr) launch_k(k_q4_window<NB>, dim3((p.maxSeq + kPT - 1) / kPT, p.G, p.B), dim3(kWThreads), WindowShape<NB>::kSmem, s, true, p);
+    const long long blocks = (long long)p.G * ((p.M + per - 1) / per + std::min(p.B, p.M) - 1);
+    // a grid that gives every block an SM of its own asks for so much shared memory that it gets one (blocks are dealt out two to an SM otherwise)
+    const size_t smem = blocks <= g_num_sms ? kAlone : PrefillShape<NB>::kSmem;
+    if (p.M > 0) launch_k(k_q4_prefill<NB>, dim3((unsigned)blocks), dim3(kPThreads), smem, s, true, p);
+    // a block's queries serve all its key tiles: about two blocks per SM
+    const int tiles = (p.maxSeq + kPT - 1) / kPT, share = std::max(1, 2 * g_num_sms / std::max(1, p.G * p.B));
+    if (p.accOut != nullptr) launch_k(k_q4_window<NB>, dim3(std::min(tiles, share), p.G, p.B), dim3(kWThreads), WindowShape<NB>::kSmem, s, true, p);
 }
 
 }  // namespace
