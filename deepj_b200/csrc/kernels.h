@@ -143,6 +143,7 @@ struct Q4LoadArgs { const unsigned char* cache; int maxSeq; const float* at; con
 struct Q4EvictArgs {
     const unsigned char* src; int srcMax; unsigned char* dst; int dstMax;
     const float* len; const float* acc; float* accOut; float* lenOut; float* kept; int B, G, hd, budget, recent;
+    float* ws;                                           // q4_evict_ws_floats
 };
 DJ_PART size_t q4_plane_bytes(int B, int G, int maxSeq, int hd);
 DJ_PART size_t q4_attn_ws_floats(const Q4AttnArgs& a);
@@ -151,6 +152,7 @@ DJ_PART void launch_q4_attn(const Q4AttnArgs& a, cudaStream_t s);               
 DJ_PART size_t q4_decode_ws_floats(const Q4AttnArgs& a);
 DJ_PART void launch_q4_decode(const Q4AttnArgs& a, cudaStream_t s);             // the same for one token of every sequence (q4_decode.cu)
 DJ_PART void launch_q4_load(const Q4LoadArgs& a, cudaStream_t s);
+DJ_PART size_t q4_evict_ws_floats(const Q4EvictArgs& a);
 DJ_PART void launch_q4_evict(const Q4EvictArgs& a, cudaStream_t s);
 
 // ── projections with bf16 weights (bf16_linear.cu, bf16_gemm_tc.cu) ──

@@ -58,14 +58,25 @@ __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
         const size_t at = (size_t)(pos + t) * (16 * NB) + 2 * e;
         c = *reinterpret_cast<const float2*>(p.cosT + at); s = *reinterpret_cast<const float2*>(p.sinT + at);
     }
-    for (int i = warp * RPW + lane / LPR; i - lane / LPR < 2 * p.G; i += 8 * RPW) {      // keys of all heads, then their values
-        const bool on = i < 2 * p.G, value = i >= p.G;
-        const int g = value ? i - p.G : i;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (on) x = *reinterpret_cast<const float4*>(src + (value ? p.v_off : p.k_off) + g * (32 * NB) + 4 * e);
-        if (!value && p.cosT != nullptr) x = q4_rotate(x, c, s);
-        unsigned char* page = p.cache + (((size_t)b * p.G + g) * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
-        q4_put_row<NB>(page, row % kQ4Page, value, e, x, on);
+    // keys of all heads, then their values, four rows of a warp at a time: their loads go out together
+    constexpr int kAhead = 4;
+#pragma unroll 1
+    for (int i0 = warp * RPW; i0 < 2 * p.G; i0 += 8 * RPW * kAhead) {
+        float4 x[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int i = i0 + k * 8 * RPW + lane / LPR;
+            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < 2 * p.G) x[k] = *reinterpret_cast<const float4*>(src + (i < p.G ? p.k_off + i * (32 * NB) : p.v_off + (i - p.G) * (32 * NB)) + 4 * e);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            if (i0 + k * 8 * RPW >= 2 * p.G) break;
+            const int i = i0 + k * 8 * RPW + lane / LPR, g = i < p.G ? i : i - p.G;
+            if (i < p.G && p.cosT != nullptr) x[k] = q4_rotate(x[k], c, s);
+            unsigned char* page = p.cache + (((size_t)b * p.G + g) * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
+            q4_put_row<NB>(page, row % kQ4Page, i >= p.G, e, x[k], i < 2 * p.G);
+        }
     }
 }
 
@@ -84,28 +95,42 @@ __global__ void __launch_bounds__(256) k_q4_load(const LoadParams p) {
     const int at = p.at != nullptr ? (int)p.at[b] : 0, end = min(p.maxSeq, p.end != nullptr ? (int)p.end[b] : p.maxSeq);
     if (at < 0) return;
     const int j = e >> 3, t = e & 3, shift = (e & 4);    // the four values are one nibble of each byte of word (t, j)
-    for (int i = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i < p.T && i < end - at; i += gridDim.x * (256 / LPR)) {
-        const int row = at + i, r = row % kQ4Page;
-        const unsigned char* page = p.cache + ((size_t)bg * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
-        const size_t to = ((size_t)bg * p.T + i) * (32 * NB) + 4 * e;
+    const int rows = min(p.T, end - at), step = gridDim.x * (256 / LPR);
+#pragma unroll 1
+    for (int i0 = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i0 < rows; i0 += 4 * step) {      // four rows at a time
+        uint32_t w[4][2];
+        float scale[4][2];
 #pragma unroll
-        for (int value = 0; value < 2; value++) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(r, t, j));
-            const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (r * NB + j) * 2));
-            auto val = [&](int k) { return (float)q4_code(w, 8 * k + shift) * s; };
-            *reinterpret_cast<float4*>((value ? p.v : p.k) + to) = make_float4(val(0), val(1), val(2), val(3));
+        for (int k = 0; k < 4; k++) {
+            const int row = at + min(i0 + k * step, rows - 1), r = row % kQ4Page;
+            const unsigned char* page = p.cache + ((size_t)bg * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
+#pragma unroll
+            for (int value = 0; value < 2; value++) {
+                w[k][value] = *reinterpret_cast<const uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(r, t, j));
+                scale[k][value] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (r * NB + j) * 2));
+            }
         }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i0 + k * step < rows) {
+                const size_t to = ((size_t)bg * p.T + i0 + k * step) * (32 * NB) + 4 * e;
+#pragma unroll
+                for (int value = 0; value < 2; value++) {
+                    auto val = [&](int n) { return (float)q4_code(w[k][value], 8 * n + shift) * scale[k][value]; };
+                    __stcs(reinterpret_cast<float4*>((value ? p.v : p.k) + to), make_float4(val(0), val(1), val(2), val(3)));
+                }
+            }
     }
 }
 
 // ───────────── eviction ─────────────
-// One block per sequence and head.  The weight of the last row that stays is found by radix selection (four passes of eight bits over an
-// order-preserving map of the floats, NaN below all), then the rows move in order: the i-th kept row is never before row i, so a block that reads
-// a run of rows before it writes it may work in place.
+// A block per sequence and head finds the weight of the last row that stays by radix selection (11, 11 and 10 bits of an order-preserving map of the
+// floats, NaN below all), and lists the rows that stay, in order; their weights move on the way.  Another kernel moves the rows: eight rows of a warp
+// at a time, so that what it writes is contiguous.  In place the rows go through the workspace: blocks that move rows of one head run in any order.
+// Bound by latency for few heads, by the rows' bytes for many.
 struct EvictParams {
-    const unsigned char* src; int srcMax, srcPages;
-    unsigned char* dst; int dstMax, dstPages;
-    const float* len; const float* acc; float* accOut; float* lenOut; float* kept;
+    const float* len; int srcMax, dstMax;
+    const float* acc; float* accOut; float* lenOut; float* kept; int* list;
     int G, budget, recent;
 };
 
@@ -116,46 +141,70 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kEvictThreads = 256;
-template <int NB>
-__global__ void __launch_bounds__(kEvictThreads) k_q4_evict(const EvictParams p) {
-    constexpr int kRowWords = 4 * NB;                    // code words of a row
-    __shared__ unsigned s_hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_need, s_scan[kEvictThreads / 32], s_from[kEvictThreads];
-    __shared__ float s_weight[kEvictThreads];
+constexpr int kEvictThreads = 512, kEvictBins = 2048;
+__global__ void __launch_bounds__(kEvictThreads) k_q4_select(const EvictParams p) {
+    __shared__ int s_bins[kEvictBins];
+    __shared__ int s_scan[kEvictThreads / 32], s_prefix, s_need;
     pdl_wait();
     pdl_launch_dependents();
     const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t bg = (size_t)b * p.G + g;
     const int n = min(max((int)p.len[b], 0), p.srcMax), stay = min(n, p.budget), recent = min(p.recent, stay), top = stay - recent, old = n - recent;
     const float* const acc = p.acc + bg * p.srcMax;
+    int* const list = p.list + bg * p.budget;
+    auto before = [&](int mine, int& total) {            // sum over the threads before this one, and over all
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+        if (lane == 31) s_scan[warp] = upto;
+        __syncthreads();
+        int sum = upto - mine;
+        total = 0;
+#pragma unroll
+        for (int k = 0; k < kEvictThreads / 32; k++) { if (k < warp) sum += s_scan[k]; total += s_scan[k]; }
+        __syncthreads();
+        return sum;
+    };
     // the key of the last old row that stays, and how many of the rows with that key do
     uint32_t prefix = 0;
     int need = top;
     if (top > 0 && top < old) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            s_hist[tid] = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 3; pass++) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t above = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10, mask = pass == 2 ? 1023u : 2047u;
+            for (int i = tid; i < kEvictBins; i += kEvictThreads) s_bins[i] = 0;
             __syncthreads();
-            for (int i = tid; i < old; i += kEvictThreads) {
-                const uint32_t key = weight_key(acc[i]);
-                if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s_hist[key >> shift & 255], 1u);
+            for (int i0 = tid; i0 < old; i0 += 4 * kEvictThreads) {
+                float w[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) w[k] = i0 + k * kEvictThreads < old ? acc[i0 + k * kEvictThreads] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t key = weight_key(w[k]);
+                    if (i0 + k * kEvictThreads < old && (key & above) == prefix) atomicAdd(&s_bins[key >> shift & mask], 1);
+                }
             }
             __syncthreads();
-            if (tid == 0) {
-                int d = 255;
-                while (d > 0 && (int)s_hist[d] < need) need -= s_hist[d--];
-                s_prefix = prefix | (uint32_t)d << shift;
-                s_need = need;
+            // bins in falling order, four to a thread: the one in which the count reaches `need`
+            int c[4], mine = 0, all;
+#pragma unroll
+            for (int k = 0; k < 4; k++) { c[k] = s_bins[kEvictBins - 1 - 4 * tid - k]; mine += c[k]; }
+            int upto = before(mine, all);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (upto < need && upto + c[k] >= need) { s_prefix = (int)(prefix | (uint32_t)(kEvictBins - 1 - 4 * tid - k) << shift); s_need = need - upto; }
+                upto += c[k];
             }
             __syncthreads();
-            prefix = s_prefix; need = s_need;
+            prefix = (uint32_t)s_prefix; need = s_need;
             __syncthreads();
         }
     }
-    const bool all = top == old;
     // in order, a run of rows at a time: which stay, and where they go
+    const bool every = top == old;
     int at = 0, ties = 0;                                // rows placed, rows of the threshold's key met
+#pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
         const int i = i0 + tid;
         float w = 0.0f;
@@ -163,62 +212,66 @@ __global__ void __launch_bounds__(kEvictThreads) k_q4_evict(const EvictParams p)
         if (i < n) {
             w = acc[i];
             const uint32_t key = weight_key(w);
-            over = i >= old || all || (top > 0 && key > prefix);
+            over = i >= old || every || (top > 0 && key > prefix);
             tie = !over && top > 0 && key == prefix;
         }
-        auto rank = [&](bool flag, int& total) {         // flags of the threads before this one, and of all
-            const unsigned m = __ballot_sync(0xffffffffu, flag);
-            if (lane == 0) s_scan[warp] = __popc(m);
-            __syncthreads();
-            int before = __popc(m & ((1u << lane) - 1)), sum = 0;
-#pragma unroll
-            for (int k = 0; k < kEvictThreads / 32; k++) { if (k < warp) before += s_scan[k]; sum += s_scan[k]; }
-            __syncthreads();
-            total = sum;
-            return before;
-        };
-        int met, found;
-        const int tieRank = ties + rank(tie, met);
-        ties += met;
-        const bool keep = over || (tie && tieRank < need);
-        const int place = rank(keep, found);
-        if (keep) { s_from[place] = i; s_weight[place] = w; }
-        __syncthreads();
-        // the run's rows: all reads come before the writes
-        for (int base = 0; base < found; base += kEvictThreads / 8) {
-            const int r = base + tid / 8, c = tid % 8;   // eight threads a row: half of a K or V row's words and scales each
-            constexpr int kPart = kRowWords / 4 > 0 ? kRowWords / 4 : 1;
-            uint32_t words[kPart];
-            unsigned short scale = 0;
-            const bool value = c >= 4;
-            const int t = c & 3;
-            const bool on = r < found;
-            if (on) {
-                const int from = s_from[r];
-                const unsigned char* page = p.src + (bg * p.srcPages + from / kQ4Page) * Q4Page<NB>::kBytes;
-                const unsigned char* piece = page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(from % kQ4Page, t, 0);
-#pragma unroll
-                for (int j = 0; j < NB; j++) words[j] = *reinterpret_cast<const uint32_t*>(piece + 4 * j);
-                if (t < NB) scale = *reinterpret_cast<const unsigned short*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (from % kQ4Page * NB + t) * 2);
-            }
-            __syncthreads();
-            if (on) {
-                const int to = at + r;
-                unsigned char* page = p.dst + (bg * p.dstPages + to / kQ4Page) * Q4Page<NB>::kBytes;
-                unsigned char* piece = page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(to % kQ4Page, t, 0);
-#pragma unroll
-                for (int j = 0; j < NB; j++) *reinterpret_cast<uint32_t*>(piece + 4 * j) = words[j];
-                if (t < NB) *reinterpret_cast<unsigned short*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (to % kQ4Page * NB + t) * 2) = scale;
-                if (c == 0) {
-                    p.accOut[bg * p.dstMax + to] = s_weight[r];
-                    if (p.kept != nullptr) p.kept[bg * p.budget + to] = (float)s_from[r];
-                }
-            }
+        // one scan for both: rows that stay in the low half, ties in the high half (runs have 512)
+        int both;
+        const int sums = before((over ? 1 : 0) + (tie ? 1 << 16 : 0), both);
+        const int tieRank = ties + (sums >> 16), taken = min(max(need - ties, 0), sums >> 16);      // of the ties before this row, those that stay
+        const int place = at + (sums & 0xffff) + taken;
+        if (over || (tie && tieRank < need)) {
+            list[place] = i;
+            p.accOut[bg * p.dstMax + place] = w;         // never behind row i: the rows of this run have been read
+            if (p.kept != nullptr) p.kept[bg * p.budget + place] = (float)i;
         }
-        __syncthreads();
-        at += found;
+        at += (both & 0xffff) + min(max(need - ties, 0), both >> 16);
+        ties += both >> 16;
     }
     if (g == 0 && tid == 0) p.lenOut[b] = (float)stay;
+}
+
+struct MoveParams {
+    const unsigned char* src; int srcPages; unsigned char* dst; int dstPages;
+    const float* len; int srcMax, budget, G;
+    const int* list;                                     // rows of the source in the destination's order, or null: the same
+    int inPlace;                                         // rows of a sequence that keeps them all stay where they are
+};
+template <int NB>
+__global__ void __launch_bounds__(256) k_q4_move(const MoveParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int g = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, t = lane & 3;
+    const size_t bg = (size_t)b * p.G + g;
+    const int n = min(max((int)p.len[b], 0), p.srcMax), stay = min(n, p.budget);
+    if (p.inPlace && n <= p.budget) return;
+    for (int to = (int)(blockIdx.x * 8 + (threadIdx.x >> 5)) * 8 + (lane >> 2); to < stay; to += gridDim.x * 64) {
+        const int from = p.list != nullptr ? p.list[bg * p.budget + to] : to, rf = from % kQ4Page, rt = to % kQ4Page;
+        const unsigned char* const s = p.src + (bg * p.srcPages + from / kQ4Page) * Q4Page<NB>::kBytes;
+        unsigned char* const d = p.dst + (bg * p.dstPages + to / kQ4Page) * Q4Page<NB>::kBytes;
+        uint32_t w[2][NB];
+        unsigned short scale[2];
+#pragma unroll
+        for (int value = 0; value < 2; value++) {
+            const unsigned char* const half = s + (value ? Q4Page<NB>::kV : 0);
+            if constexpr (NB == 4) { const uint4 v = *reinterpret_cast<const uint4*>(half + Q4Page<NB>::word(rf, t, 0)); w[value][0] = v.x; w[value][1] = v.y; w[value][2] = v.z; w[value][3] = v.w; }
+            else {
+#pragma unroll
+                for (int j = 0; j < NB; j++) w[value][j] = *reinterpret_cast<const uint32_t*>(half + Q4Page<NB>::word(rf, t, j));
+            }
+            scale[value] = t < NB ? *reinterpret_cast<const unsigned short*>(half + Q4Page<NB>::kKs + (rf * NB + t) * 2) : 0;
+        }
+#pragma unroll
+        for (int value = 0; value < 2; value++) {
+            unsigned char* const half = d + (value ? Q4Page<NB>::kV : 0);
+            if constexpr (NB == 4) *reinterpret_cast<uint4*>(half + Q4Page<NB>::word(rt, t, 0)) = make_uint4(w[value][0], w[value][1], w[value][2], w[value][3]);
+            else {
+#pragma unroll
+                for (int j = 0; j < NB; j++) *reinterpret_cast<uint32_t*>(half + Q4Page<NB>::word(rt, t, j)) = w[value][j];
+            }
+            if (t < NB) *reinterpret_cast<unsigned short*>(half + Q4Page<NB>::kKs + (rt * NB + t) * 2) = scale[value];
+        }
+    }
 }
 
 template <int NB> void append(const AppendParams& p, cudaStream_t s) { launch_k(k_q4_append<NB>, dim3(p.M), dim3(256), 0, s, true, p); }
@@ -226,7 +279,13 @@ template <int NB> void load(const LoadParams& p, cudaStream_t s) {
     const int per = 256 / (8 * NB), blocks = std::min((p.T + per - 1) / per, std::max(1, 16 * g_num_sms / (p.B * p.G)));
     launch_k(k_q4_load<NB>, dim3(blocks, p.B * p.G), dim3(256), 0, s, true, p);
 }
-template <int NB> void evict(const EvictParams& p, int B, cudaStream_t s) { launch_k(k_q4_evict<NB>, dim3(p.G, B), dim3(kEvictThreads), 0, s, true, p); }
+template <int NB> void move(const MoveParams& p, int B, cudaStream_t s) {
+    const int most = std::max(1, 8 * 8 * g_num_sms / (p.G * B));         // blocks of a head: all heads' fill the chip some times over
+    launch_k(k_q4_move<NB>, dim3(std::min((p.budget + 63) / 64, most), p.G, B), dim3(256), 0, s, true, p);
+}
+void move_rows(const MoveParams& p, int B, int hd, cudaStream_t s) {
+    if (hd == 128) move<4>(p, B, s); else if (hd == 64) move<2>(p, B, s); else move<1>(p, B, s);
+}
 
 }  // namespace
 
@@ -241,10 +300,21 @@ void launch_q4_load(const Q4LoadArgs& a, cudaStream_t s) {
     LoadParams p = {a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.at, a.end, a.k, a.v, a.B, a.G, a.T};
     if (a.hd == 128) load<4>(p, s); else if (a.hd == 64) load<2>(p, s); else load<1>(p, s);
 }
+// In place: the rows that stay, in pages as well.  The list of rows follows.
+static size_t evict_pages_floats(const Q4EvictArgs& a) { return a.src == a.dst ? (q4_plane_bytes(a.B, a.G, a.budget, a.hd) + 3) / 4 : 0; }
+size_t q4_evict_ws_floats(const Q4EvictArgs& a) { return evict_pages_floats(a) + (size_t)a.B * a.G * a.budget; }
 void launch_q4_evict(const Q4EvictArgs& a, cudaStream_t s) {
-    EvictParams p = {a.src, a.srcMax, (a.srcMax + kQ4Page - 1) / kQ4Page, a.dst, a.dstMax, (a.dstMax + kQ4Page - 1) / kQ4Page,
-                     a.len, a.acc, a.accOut, a.lenOut, a.kept, a.G, a.budget, a.recent};
-    if (a.hd == 128) evict<4>(p, a.B, s); else if (a.hd == 64) evict<2>(p, a.B, s); else evict<1>(p, a.B, s);
+    int* const list = reinterpret_cast<int*>(a.ws + evict_pages_floats(a));
+    EvictParams p = {a.len, a.srcMax, a.dstMax, a.acc, a.accOut, a.lenOut, a.kept, list, a.G, a.budget, a.recent};
+    launch_k(k_q4_select, dim3(a.G, a.B), dim3(kEvictThreads), 0, s, true, p);
+    auto pages = [](int rows) { return (rows + kQ4Page - 1) / kQ4Page; };
+    const bool inPlace = a.src == a.dst;
+    unsigned char* const between = reinterpret_cast<unsigned char*>(a.ws);
+    MoveParams m = {a.src, pages(a.srcMax), inPlace ? between : a.dst, pages(inPlace ? a.budget : a.dstMax), a.len, a.srcMax, a.budget, a.G, list, inPlace};
+    move_rows(m, a.B, a.hd, s);
+    if (!inPlace) return;
+    m.src = between; m.srcPages = pages(a.budget); m.dst = a.dst; m.dstPages = pages(a.dstMax); m.list = nullptr;
+    move_rows(m, a.B, a.hd, s);
 }
 
 }  // namespace dj

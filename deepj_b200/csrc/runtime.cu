@@ -787,6 +787,7 @@ void do_op(Ctx& ctx, const int32_t* c) {
             a.len = f32(ctx, c[4], a.B, what);
             a.acc = f32(ctx, c[5], sz(a.B, a.G) * a.srcMax, what); a.accOut = f32(ctx, c[9], sz(a.B, a.G) * a.dstMax, what);
             a.lenOut = f32(ctx, c[10], a.B, what); a.kept = f32_opt(ctx, c[11], sz(a.B, a.G) * a.budget, what);
+            a.ws = scratch(q4_evict_ws_floats(a));
             if (go) launch_q4_evict(a, s);
             break;
         }
