@@ -145,39 +145,52 @@ __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, i
 }
 
 // Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 8·NB lanes of four values each; `place(row, m, head, position)` says
-// which one row `row` is (false: zeros).  factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).
+// which one row `row` is, and whether it is one (false: zeros, but the place can be read).  factors[row] makes a sum of products a score in log2 units
+// (NaN where the row holds an infinity or a NaN).  Four rows' loads go out together: one after another they took 20000 cycles a tile.
 template <int NB, typename Place>
 __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, Place place) {
-    constexpr int HD = 32 * NB, LPR = 8 * NB, RPW = 32 / LPR;
+    constexpr int HD = 32 * NB, LPR = 8 * NB, RPW = 32 / LPR, AHEAD = 4;
     const int e = lane % LPR;
     // this lane's dims 4e … 4e + 3 in the tiles' order: (0, 2) and (1, 3), eight bytes apart
     const int piece = (e >> 3) * 4 + (e & 3), at = (piece >> 3) * (kPT * 128) + (e & 4);
-#pragma unroll 4
-    for (int r = warp * RPW + lane / LPR; r < kPT; r += warps * RPW) {
-        int m, head, position;
-        const bool on = place(r, m, head, position);
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (on) {
-            const size_t tab = (size_t)position * (HD / 2) + 2 * e;
-            x = q4_rotate(*reinterpret_cast<const float4*>(p.qkv + (size_t)m * p.ld + p.q_off + head * HD + 4 * e), *reinterpret_cast<const float2*>(p.cosT + tab),
-                          *reinterpret_cast<const float2*>(p.sinT + tab));
-        }
-        float most = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), bad = (x.x + x.y + x.z + x.w) * 0.0f;
+#pragma unroll 1
+    for (int r0 = warp * RPW + lane / LPR; r0 < kPT; r0 += AHEAD * warps * RPW) {
+        float4 x[AHEAD];
+        float2 cs[AHEAD], sn[AHEAD];
+        bool on[AHEAD];
 #pragma unroll
-        for (int o = 1; o < LPR; o <<= 1) { most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o)); bad += __shfl_xor_sync(0xffffffffu, bad, o); }
-        // the largest value comes to 256 … 512
-        most = fmaxf(most, 7.8886091e-31f);
-        const int bits = __float_as_int(most) & 0x7f800000;
-        const bool fine = bad == 0.0f && most < 1e30f;
-        const float mul = fine ? __int_as_float(0x7f000000 - bits) * 256.0f : 0.0f;
-        if (!fine) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        uint2 h, l;
-        split_half(x.x * mul, x.z * mul, h.x, l.x);
-        split_half(x.y * mul, x.w * mul, h.y, l.y);
-        const int to = at + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-        *reinterpret_cast<uint32_t*>(hi + to) = h.x; *reinterpret_cast<uint32_t*>(hi + to + 8) = h.y;
-        *reinterpret_cast<uint32_t*>(lo + to) = l.x; *reinterpret_cast<uint32_t*>(lo + to + 8) = l.y;
-        if (e == 0) factors[r] = fine ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
+        for (int k = 0; k < AHEAD; k++) {
+            int m, head, position;
+            on[k] = place(min(r0 + k * warps * RPW, kPT - 1), m, head, position);
+            const size_t tab = (size_t)position * (HD / 2) + 2 * e;
+            x[k] = *reinterpret_cast<const float4*>(p.qkv + (size_t)m * p.ld + p.q_off + head * HD + 4 * e);
+            cs[k] = *reinterpret_cast<const float2*>(p.cosT + tab);
+            sn[k] = *reinterpret_cast<const float2*>(p.sinT + tab);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const int r = r0 + k * warps * RPW;
+            float4 y = q4_rotate(x[k], cs[k], sn[k]);
+            if (!on[k]) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float most = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
+            if ((y.x + y.y + y.z + y.w) * 0.0f != 0.0f) most = INFINITY;
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // the largest value comes to 256 … 512
+            most = fmaxf(most, 7.8886091e-31f);
+            const int bits = __float_as_int(most) & 0x7f800000;
+            const bool fine = most < 1e30f;
+            const float mul = fine ? __int_as_float(0x7f000000 - bits) * 256.0f : 0.0f;
+            if (!fine) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            uint2 h, l;
+            split_half(y.x * mul, y.z * mul, h.x, l.x);
+            split_half(y.y * mul, y.w * mul, h.y, l.y);
+            if (r >= kPT) break;
+            const int to = at + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+            *reinterpret_cast<uint32_t*>(hi + to) = h.x; *reinterpret_cast<uint32_t*>(hi + to + 8) = h.y;
+            *reinterpret_cast<uint32_t*>(lo + to) = l.x; *reinterpret_cast<uint32_t*>(lo + to + 8) = l.y;
+            if (e == 0) factors[r] = fine ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
+        }
     }
 }
 
@@ -266,18 +279,19 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     const int used = max(0, min(tokensPerTile, room - t0));              // tokens of this tile
     const int keys = used > 0 ? len + t0 + used : 0, tiles = (keys + kKT - 1) / kKT, pages = (keys + kQ4Page - 1) / kQ4Page;
 
+    const int inverse = 65535 / p.ratio + 1;      // r · inverse / 2^16 is r / ratio for a row r of the tile
     auto queries = [&]() {                        // twelve warps lay the queries down
         query_rows<NB>(p, warp, 12, lane, smem, smem + S::kQ, s_factor, [&](int r, int& qm, int& qh, int& qp) {
-            const int t = r / p.ratio;
-            qm = first + t0 + t; qh = g * p.ratio + r - t * p.ratio; qp = pos + t0 + t;
-            return t < used;
+            const int t = min(r * inverse >> 16, used - 1);
+            qm = first + t0 + t; qh = g * p.ratio + min(r - t * p.ratio, p.ratio - 1); qp = pos + t0 + t;
+            return r < used * p.ratio;
         });
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(qReady);
     };
     if (warp < 4) {
-        const int row = tid, token = row / p.ratio, head = g * p.ratio + row % p.ratio;
+        const int row = tid, token = row * inverse >> 16, head = g * p.ratio + row - token * p.ratio;
         const bool on = token < used;
         const int m = first + t0 + token, last = on ? len + t0 + token : -1;      // the row's place in the buffers, its newest key
         float c = 1.0f, top = -INFINITY;
@@ -377,12 +391,12 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 }
             }
             __syncwarp();                         // a warp stores the rows that it has staged
-#pragma unroll 4
-            for (int i = lane / LPR; ok && i < 32; i += RPW) {
-                const int r = warp * 32 + i, t = r / p.ratio, e = lane % LPR;
-                if (t < used)
-                    *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) =
-                        *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
+            const int rows = min(32, used * p.ratio - warp * 32), e = lane % LPR;
+#pragma unroll 8
+            for (int i = lane / LPR; i < rows; i += RPW) {
+                const int r = warp * 32 + i, t = r * inverse >> 16;
+                const float4 v = *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
+                if (ok) *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) = v;
             }
             if (on && p.stats != nullptr && t0 + token >= room - p.window)
                 *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
@@ -542,8 +556,8 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
                 const int n = min(rows - r0, kPT);
                 if (k0 == (int)blockIdx.x * kPT || rows > kPT) {         // the queries stay for all tiles if one tile holds them
                     query_rows<NB>(p, warp, 4, lane, smem, smem + S::kTile, s_factor, [&](int i, int& qm, int& qh, int& qp) {
-                        const int of = (r0 + i) / p.ratio, token = room - window + of;
-                        qm = first + token; qh = g * p.ratio + r0 + i - of * p.ratio; qp = pos + token;
+                        const int row = r0 + min(i, n - 1), of = row / p.ratio, token = room - window + of;
+                        qm = first + token; qh = g * p.ratio + row - of * p.ratio; qp = pos + token;
                         return i < n;
                     });
                     __syncthreads();
