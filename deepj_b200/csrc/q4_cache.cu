@@ -15,7 +15,7 @@ struct AppendParams {
     const float* src; int k_off, v_off, ld;
     unsigned char* cache; int maxSeq, pages;
     const float* starts; const float* len; const float* pos; const float* cosT; const float* sinT; int maxPos;
-    int B, G, T, M;
+    int B, G, T, M, share;                               // share: warps of a row (a power of two up to eight)
 };
 
 // The sequence that packed row m belongs to (the first, should ranges overlap), or -1; whole warps call it.
@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
     constexpr int LPR = 8 * NB, RPW = 32 / LPR;          // lanes of a row, rows of a warp
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = blockIdx.x;
+    const int lane = threadIdx.x & 31, at = blockIdx.x * 8 + (threadIdx.x >> 5), m = at / p.share, part = at - m * p.share;
+    if (m >= p.M) return;
     int first = 0, tokens = p.T, b;
     if (p.starts != nullptr) {
         b = sequence_of(p.starts, p.B, p.M, m, lane, first, tokens);
@@ -61,18 +62,18 @@ __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
     // keys of all heads, then their values, four rows of a warp at a time: their loads go out together
     constexpr int kAhead = 4;
 #pragma unroll 1
-    for (int i0 = warp * RPW; i0 < 2 * p.G; i0 += 8 * RPW * kAhead) {
+    for (int i0 = part * RPW; i0 < 2 * p.G; i0 += p.share * RPW * kAhead) {
         float4 x[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
-            const int i = i0 + k * 8 * RPW + lane / LPR;
+            const int i = i0 + k * p.share * RPW + lane / LPR;
             x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (i < 2 * p.G) x[k] = *reinterpret_cast<const float4*>(src + (i < p.G ? p.k_off + i * (32 * NB) : p.v_off + (i - p.G) * (32 * NB)) + 4 * e);
         }
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
-            if (i0 + k * 8 * RPW >= 2 * p.G) break;
-            const int i = i0 + k * 8 * RPW + lane / LPR, g = i < p.G ? i : i - p.G;
+            if (i0 + k * p.share * RPW >= 2 * p.G) break;
+            const int i = i0 + k * p.share * RPW + lane / LPR, g = i < p.G ? i : i - p.G;
             if (i < p.G && p.cosT != nullptr) x[k] = q4_rotate(x[k], c, s);
             unsigned char* page = p.cache + (((size_t)b * p.G + g) * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
             q4_put_row<NB>(page, row % kQ4Page, i >= p.G, e, x[k], i < 2 * p.G);
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(256) k_q4_move(const MoveParams p) {
     }
 }
 
-template <int NB> void append(const AppendParams& p, cudaStream_t s) { launch_k(k_q4_append<NB>, dim3(p.M), dim3(256), 0, s, true, p); }
+template <int NB> void append(const AppendParams& p, cudaStream_t s) { launch_k(k_q4_append<NB>, dim3((unsigned)(((long long)p.M * p.share + 7) / 8)), dim3(256), 0, s, true, p); }
 template <int NB> void load(const LoadParams& p, cudaStream_t s) {
     const int per = 256 / (8 * NB), blocks = std::min((p.T + per - 1) / per, std::max(1, 16 * g_num_sms / (p.B * p.G)));
     launch_k(k_q4_load<NB>, dim3(blocks, p.B * p.G), dim3(256), 0, s, true, p);
@@ -292,7 +293,9 @@ void move_rows(const MoveParams& p, int B, int hd, cudaStream_t s) {
 size_t q4_plane_bytes(int B, int G, int maxSeq, int hd) { return (size_t)B * G * ((maxSeq + kQ4Page - 1) / kQ4Page) * kQ4PageBytes * (hd / 32); }
 
 void launch_q4_append(const Q4AttnArgs& a, int T, cudaStream_t s) {
-    AppendParams p = {a.qkv, a.k_off, a.v_off, a.ld, a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.starts, a.len, a.pos, a.cosT, a.sinT, a.maxPos, a.B, a.G, T, a.M};
+    AppendParams p = {a.qkv, a.k_off, a.v_off, a.ld, a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.starts, a.len, a.pos, a.cosT, a.sinT, a.maxPos, a.B, a.G, T, a.M, 1};
+    // few rows are shared by warps; with one warp to a row the place of a row is looked up once and its heads' loads follow one another
+    while (p.share < 8 && (long long)a.M * p.share < 24 * g_num_sms) p.share *= 2;
     if (a.hd == 128) append<4>(p, s); else if (a.hd == 64) append<2>(p, s); else append<1>(p, s);
 }
 void launch_q4_load(const Q4LoadArgs& a, cudaStream_t s) {
