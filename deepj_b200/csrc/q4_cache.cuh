@@ -42,13 +42,24 @@ __device__ __forceinline__ uint32_t q4_codes(const float4& x, float& scale) {
     most = most == most ? most : 0.0f;
     const float s = fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(most * (1.0f / 7.0f))), kQ4ScaleMin), kQ4ScaleMax), inverse = __frcp_rn(s);
     scale = most > 0.0f ? s : 0.0f;
-    const float q[4] = {x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse};
+    // the sum with 1.5 · 2^23 ends in the rounded quotient, in two's complement
+    uint32_t codes = 0;
     float off = 0.0f;                             // the largest distance from a whole number
+    const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 4; i++) off = fmaxf(off, fabsf(q[i] - ((q[i] + 12582912.0f) - 12582912.0f)));
-    auto code = [](float v) { return (uint32_t)min(max(__float2int_rn(v), -7), 7) & 15u; };     // NaN → 0
-    if (__any_sync(0xffffffffu, off > 0.4999f)) return code(x.x / s) | code(x.y / s) << 8 | code(x.z / s) << 16 | code(x.w / s) << 24;
-    return code(q[0]) | code(q[1]) << 8 | code(q[2]) << 16 | code(q[3]) << 24;
+    for (int i = 0; i < 4; i++) {
+        const float q = v[i] * inverse, sum = q + 12582912.0f;
+        off = fmaxf(off, fabsf(q - (sum - 12582912.0f)));
+        codes |= ((uint32_t)__float_as_int(sum) & 15u) << (8 * i);
+    }
+    // blocks that saturate, NaN and infinities take this way too
+    const float all = (v[0] + v[1]) + (v[2] + v[3]);
+    if (__any_sync(0xffffffffu, off > 0.4999f || most > 7.0f * kQ4ScaleMax || all != all)) {
+        codes = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) codes |= ((uint32_t)min(max(__float2int_rn(v[i] / s), -7), 7) & 15u) << (8 * i);      // NaN → 0
+    }
+    return codes;
 }
 
 // 8·NB consecutive lanes (all lanes of the warp are here) put one row into its page: lane e of them holds the values 4e … 4e + 3.
