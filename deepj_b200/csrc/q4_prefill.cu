@@ -374,7 +374,9 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         }
         if (tiles > 0) {
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
-            ok = __all_sync(0xffffffffu, ok && mbar_wait_long(vEmpty, (tiles - 1) & 1, &s_abort, p.error, 343));
+            // the last scores are there once P·V of tiles - 3 is done: the wait for the next one keeps the parities apart
+            ok = __all_sync(0xffffffffu, ok && (tiles < 2 || mbar_wait_long(vEmpty, (tiles - 2) & 1, &s_abort, p.error, 343)) &&
+                                             mbar_wait_long(vEmpty, (tiles - 1) & 1, &s_abort, p.error, 343));
             tc_fence_after();
             const float sum = sums.x + sums.y, inv = 1.0f / sum;
             constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;
