@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);      // B MN-major
     constexpr uint32_t kO = 2 * kKT;              // O's first column
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long s_bar[8 + 9];
+    __shared__ __align__(8) unsigned long long s_bar[8 + 10];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ float s_factor[kPT];
@@ -256,12 +256,14 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     const uint32_t kFull = bar(8), kEmpty = bar(9), vFull = bar(10), vEmpty = bar(11);      // one phase a tile; bars 0-7: the conversion warps' copies
     auto sFull = [&](int s) { return bar(12 + s); };
     auto pReady = [&](int s) { return bar(14 + s); };
-    const uint32_t qReady = bar(16);
+    // done: the last product.  Its phase of vEmpty cannot be waited for by those that may not have seen the one before: parities name two phases.
+    const uint32_t qReady = bar(16), done = bar(17);
     if (tid == 0) {
         for (int s = 0; s < 8; s++) mbar_init(bar(s), 1);
         mbar_init(kFull, 4); mbar_init(kEmpty, 1); mbar_init(vFull, 4); mbar_init(vEmpty, 1);
         for (int s = 0; s < 2; s++) { mbar_init(sFull(s), 1); mbar_init(pReady(s), 4); }
         mbar_init(qReady, 12);
+        mbar_init(done, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -374,9 +376,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         }
         if (tiles > 0) {
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
-            // the last scores are there once P·V of tiles - 3 is done: the wait for the next one keeps the parities apart
-            ok = __all_sync(0xffffffffu, ok && (tiles < 2 || mbar_wait_long(vEmpty, (tiles - 2) & 1, &s_abort, p.error, 343)) &&
-                                             mbar_wait_long(vEmpty, (tiles - 1) & 1, &s_abort, p.error, 343));
+            ok = __all_sync(0xffffffffu, ok && mbar_wait_long(done, 0, &s_abort, p.error, 343));
             tc_fence_after();
             const float sum = sums.x + sums.y, inv = 1.0f / sum;
             constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;
@@ -484,6 +484,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 }
                 umma_commit_by(lead, vEmpty);
             }
+            umma_commit_by(lead, done);
         }
         __syncwarp();
     }
