@@ -13,6 +13,7 @@
 // The chain from scores over weights to values leaves every unit idle most of the time, and a satisfied wait on a barrier costs 170 cycles: two blocks
 // share an SM (half of its tensor and shared memory each: two S/P buffers of 64 columns, O, one tile of keys and one of values).  One block per SM with
 // tiles of 128 keys and two of each took 3900 cycles for 128 keys, where the MMAs take 2048.
+// Where tiles of queries are few, up to four blocks (a cluster) share the keys of one and join their outputs through shared memory, a part of the rows each.
 // Every wait is bounded (codes 341-350 in the device error word).
 #include <algorithm>
 #include <cmath>
@@ -37,7 +38,9 @@ struct PrefillParams {
     float* stats; int window;                     // [M][H][2] maximum (log2) and sum of the last `window` tokens' rows, or null
     const float* acc; float* accOut;
     int* error;
+    int splits, least;                            // blocks (a cluster) that share the keys of a tile of queries, tiles of keys to one at least
 };
+constexpr int kMaxSplits = 4;
 
 constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
 template <int NB> struct PrefillShape {
@@ -209,6 +212,26 @@ __device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// what block `rank` of the cluster holds at this block's address
+__device__ __forceinline__ uint32_t peer_address(uint32_t at, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float2 peer_float2(uint32_t at, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_address(at, rank)));
+    return v;
+}
+__device__ __forceinline__ float4 peer_float4(uint32_t at, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_address(at, rank)));
+    return v;
+}
+
 // Sequence, its place and the first token of query tile `tile`, the last tile of a sequence first; whole warps call it.
 __device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int tokensPerTile, int lane, int& b, int& first, int& tokens, int& t0, int& len, int& pos) {
     for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -249,10 +272,12 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ float s_factor[kPT];
+    __shared__ float2 s_row[kPT];                 // a row's maximum and sum, for the other blocks of the cluster
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
     auto bar = [&](int i) { return smem_u32(&s_bar[i]); };
+    constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;         // rows on their way out: floats of one, lanes of one, rows of a warp
     const uint32_t kFull = bar(8), kEmpty = bar(9), vFull = bar(10), vEmpty = bar(11);      // one phase a tile; bars 0-7: the conversion warps' copies
     auto sFull = [&](int s) { return bar(12 + s); };
     auto pReady = [&](int s) { return bar(14 + s); };
@@ -275,11 +300,15 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     pdl_wait();
     pdl_launch_dependents();
 
-    const int g = blockIdx.x % p.G, tokensPerTile = kPT / p.ratio;
+    const int work = blockIdx.x / p.splits, rank = blockIdx.x - work * p.splits, g = work % p.G, tokensPerTile = kPT / p.ratio;
     int b = 0, first = 0, tokens = 0, t0 = 0, len = 0, pos = 0, room = 0;
-    if (tile_of(p, blockIdx.x / p.G, tokensPerTile, lane, b, first, tokens, t0, len, pos)) room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
+    if (tile_of(p, work / p.G, tokensPerTile, lane, b, first, tokens, t0, len, pos)) room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
     const int used = max(0, min(tokensPerTile, room - t0));              // tokens of this tile
-    const int keys = used > 0 ? len + t0 + used : 0, tiles = (keys + kKT - 1) / kKT, pages = (keys + kQ4Page - 1) / kQ4Page;
+    const int keys = used > 0 ? len + t0 + used : 0, allTiles = (keys + kKT - 1) / kKT;
+    // this block's share: tiles from skip on, its keys, pages and tiles count from there
+    const int parts = p.splits > 1 ? min(p.splits, max(1, allTiles / p.least)) : 1;
+    const int skip = rank < parts ? allTiles * rank / parts : 0, tiles = rank < parts ? allTiles * (rank + 1) / parts - skip : 0;
+    const int pages = (keys + kQ4Page - 1) / kQ4Page - 2 * skip;
 
     const int inverse = 65535 / p.ratio + 1;      // r · inverse / 2^16 is r / ratio for a row r of the tile
     auto queries = [&]() {                        // twelve warps lay the queries down
@@ -295,7 +324,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     if (warp < 4) {
         const int row = tid, token = row * inverse >> 16, head = g * p.ratio + row - token * p.ratio;
         const bool on = token < used;
-        const int m = first + t0 + token, last = on ? len + t0 + token : -1;      // the row's place in the buffers, its newest key
+        const int m = first + t0 + token, last = on ? len + t0 + token - skip * kKT : -1;         // the row's place in the buffers, its newest key
         float c = 1.0f, top = -INFINITY;
         float2 sums = make_float2(0.0f, 0.0f);
         if (tiles > 0) {
@@ -378,8 +407,8 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
             ok = __all_sync(0xffffffffu, ok && mbar_wait_long(done, 0, &s_abort, p.error, 343));
             tc_fence_after();
-            const float sum = sums.x + sums.y, inv = 1.0f / sum;
-            constexpr int PITCH = HD + 4, LPR = 8 * NB, RPW = 32 / LPR;
+            const float sum = sums.x + sums.y, inv = parts > 1 ? 1.0f : 1.0f / sum;
+            if (parts > 1) s_row[row] = make_float2(top, sum);
             float* const stage = reinterpret_cast<float*>(smem);
 #pragma unroll 1
             for (int k = 0; ok && k < HD; k += 32) {
@@ -393,14 +422,14 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 }
             }
             __syncwarp();                         // a warp stores the rows that it has staged
-            const int rows = min(32, used * p.ratio - warp * 32), e = lane % LPR;
+            const int rows = parts > 1 ? 0 : min(32, used * p.ratio - warp * 32), e = lane % LPR;
 #pragma unroll 8
             for (int i = lane / LPR; i < rows; i += RPW) {
                 const int r = warp * 32 + i, t = r * inverse >> 16;
                 const float4 v = *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
                 if (ok) *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) = v;
             }
-            if (on && p.stats != nullptr && t0 + token >= room - p.window)
+            if (parts == 1 && on && p.stats != nullptr && t0 + token >= room - p.window)
                 *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
         }
     } else if (warp < 12) {
@@ -409,7 +438,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         unsigned char* const raw_at = smem + S::kRawAt + (warp - 4) * S::kRaw;
         unsigned char* const tile = smem + (value ? S::kVAt : S::kKAt);
         const uint32_t arrived = bar(warp - 4);
-        const unsigned char* from = p.cache + (((size_t)b * p.G + g) * p.pages + (w >> 1)) * Q4Page<NB>::kBytes + (value ? Q4Page<NB>::kV : 0);
+        const unsigned char* from = p.cache + (((size_t)b * p.G + g) * p.pages + 2 * skip + (w >> 1)) * Q4Page<NB>::kBytes + (value ? Q4Page<NB>::kV : 0);
         auto request = [&](int j) {               // this warp's rows of tile j
             if (lane == 0 && j < tiles && 2 * j + (w >> 1) < pages) {
                 const unsigned char* const page = from + (size_t)(2 * j) * Q4Page<NB>::kBytes;
@@ -487,6 +516,46 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             umma_commit_by(lead, done);
         }
         __syncwarp();
+    }
+    if (p.splits > 1) {
+        // every block of the cluster joins a part of the rows: Σ 2^(mᵢ − m)·Oᵢ over the sum of the same with the sums of weights
+        __syncwarp();
+        cluster_sync();
+        if (parts > 1 && rank < parts && !s_abort) {
+            const uint32_t stage = base, state = smem_u32(s_row);
+            const int all = used * p.ratio, r1 = all * (rank + 1) / parts, e = lane % LPR;
+#pragma unroll 2
+            for (int r = all * rank / parts + warp * RPW + lane / LPR; r < r1; r += (kPThreads / 32) * RPW) {
+                float2 of[kMaxSplits];
+                float4 o[kMaxSplits];
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kMaxSplits; i++) {
+                    of[i] = make_float2(-INFINITY, 0.0f);
+                    o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (i < parts) {
+                        of[i] = peer_float2(state + r * 8, i);
+                        o[i] = peer_float4(stage + (r * PITCH + 4 * e) * 4, i);
+                    }
+                    top = fmaxf(top, of[i].x);
+                }
+                float sum = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < kMaxSplits; i++) {
+                    const float f = top > -INFINITY ? ex2(of[i].x - top) : 1.0f;      // no maximum: a row of NaN
+                    sum = fmaf(of[i].y, f, sum);
+                    v.x = fmaf(o[i].x, f, v.x); v.y = fmaf(o[i].y, f, v.y); v.z = fmaf(o[i].z, f, v.z); v.w = fmaf(o[i].w, f, v.w);
+                }
+                const float inv = 1.0f / sum;
+                const int t = r * inverse >> 16, head = g * p.ratio + r - t * p.ratio;
+                const size_t m = first + t0 + t;
+                *reinterpret_cast<float4*>(p.out + m * p.ldo + head * HD + 4 * e) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                if (e == 0 && p.stats != nullptr && t0 + t >= room - p.window) *reinterpret_cast<float2*>(p.stats + (m * p.H + head) * 2) = make_float2(top, sum);
+            }
+        }
+        __syncwarp();
+        cluster_sync();                           // the rows have been read
     }
     tc_fence_before();
     __syncthreads();
@@ -609,6 +678,22 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
     if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem, 128); }
 }
 
+// Clusters of n blocks that the device holds at once with one block to an SM.
+template <int NB>
+long long resident(int n) {
+    static int most[kMaxSplits + 1] = {};
+    if (most[n] == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = n; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(n); cfg.blockDim = dim3(kPThreads); cfg.dynamicSmemBytes = kAlone; cfg.attrs = &attr; cfg.numAttrs = 1;
+        DJ_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&most[n], k_q4_prefill<NB>, &cfg));
+        most[n] = std::max(most[n], 1);
+    }
+    return most[n];
+}
+
 template <int NB>
 void prefill(const PrefillParams& p, cudaStream_t s) {
     static bool attr = false;
@@ -619,9 +704,21 @@ void prefill(const PrefillParams& p, cudaStream_t s) {
     }
     const int per = kPT / p.ratio;                // tokens of a tile; a sequence has at most one that is not full
     const long long blocks = (long long)p.G * ((p.M + per - 1) / per + std::min(p.B, p.M) - 1);
+    PrefillParams q = p;
+    // Few blocks share their keys in clusters, as far as all are resident: a block takes 0.97 µs for a tile (64 values a row) with an SM to itself, two on
+    // one 1.48.  A second wave costs more than it gives (96 blocks of 300 queries before 3300 keys: 82 µs alone, 64 by twos, 69 by threes, of which 90 fit).
+    // Joining takes some 3 µs: four tiles to a block at least, five where two are on an SM (512 queries of 32 heads × 128: 37 µs, with fours 41).
+    bool alone = blocks <= g_num_sms;
+    double best = alone ? 1.0 : 1.5;
+    for (int n = 2; n <= kMaxSplits; n++)
+        for (int two = 0; two < 2; two++) {
+            const int least = two ? 5 : 4, parts = std::min(n, p.maxSeq / (least * kKT));
+            const double cost = (two ? 1.5 : 1.0) / parts;
+            if (parts > 1 && cost < best && blocks <= (two + 1) * resident<NB>(n)) { best = cost; alone = !two; q.splits = n; q.least = least; }
+        }
     // a grid that gives every block an SM of its own asks for so much shared memory that it gets one (blocks are dealt out two to an SM otherwise)
-    const size_t smem = blocks <= g_num_sms ? kAlone : PrefillShape<NB>::kSmem;
-    if (p.M > 0) launch_k(k_q4_prefill<NB>, dim3((unsigned)blocks), dim3(kPThreads), smem, s, true, p);
+    const size_t smem = alone ? kAlone : PrefillShape<NB>::kSmem;
+    if (p.M > 0) launch_k_cluster(k_q4_prefill<NB>, dim3((unsigned)(blocks * q.splits)), dim3(kPThreads), smem, s, dim3(q.splits), q);
     // a block's queries serve all its key tiles: about two blocks per SM
     const int tiles = (p.maxSeq + kPT - 1) / kPT, share = std::max(1, 2 * g_num_sms / std::max(1, p.G * p.B));
     if (p.accOut != nullptr) launch_k(k_q4_window<NB>, dim3(std::min(tiles, share), p.G, p.B), dim3(kWThreads), WindowShape<NB>::kSmem, s, true, p);
@@ -634,7 +731,7 @@ size_t q4_attn_ws_floats(const Q4AttnArgs& a) { return a.accOut != nullptr ? (si
 void launch_q4_attn(const Q4AttnArgs& a, cudaStream_t s) {
     PrefillParams p = {a.qkv, a.q_off, a.ld, a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.starts, a.len, a.pos, a.cosT, a.sinT, a.maxPos, a.out, a.ldo,
                        a.B, a.H, a.G, a.H / a.G, a.M, (float)(1.0 / std::sqrt((double)a.hd) * 1.4426950408889634), a.accOut != nullptr ? a.ws : nullptr, a.window,
-                       a.acc, a.accOut, g_dev_error};
+                       a.acc, a.accOut, g_dev_error, 1, 1};
     if (a.M > 0) launch_q4_append(a, 1, s);
     if (a.hd == 128) prefill<4>(p, s); else if (a.hd == 64) prefill<2>(p, s); else prefill<1>(p, s);
 }
