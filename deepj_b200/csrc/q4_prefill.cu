@@ -38,9 +38,14 @@ struct PrefillParams {
     float* stats; int window;                     // [M][H][2] maximum (log2) and sum of the last `window` tokens' rows, or null
     const float* acc; float* accOut;
     int* error;
+    float* totals;                                // [block][128][hd] for the blocks of clusters
     int splits, least;                            // blocks (a cluster) that share the keys of a tile of queries, tiles of keys to one at least
 };
 constexpr int kMaxSplits = 4;
+// Tiles whose values are summed in tensor memory.  Those sums are cut off, not rounded: values of one sign lose 5.6e-9 of their sum a key, 3.4e-5 at 6000 keys.
+// So a sum of 16 tiles goes to memory, where it is added rounded: 6e-6 at any length (32 tiles: 1.1e-5), for 3 % of the time at 1500 keys and 6 % at 6000
+// (emptied every 8 tiles: 12 % and 14 %).
+constexpr int kSegment = 16;
 
 constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
 template <int NB> struct PrefillShape {
@@ -272,7 +277,12 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ float s_factor[kPT];
+    // what the loops need seldom or only behind them, so that it takes no registers
+    __shared__ float* s_out[kPT];                 // a row's place in the output; null: no row of a token
+    __shared__ int s_stat[kPT];                   // and in the statistics, or -1
+    __shared__ float s_since[kPT];                // what a row's total has to be multiplied by
     __shared__ float2 s_row[kPT];                 // a row's maximum and sum, for the other blocks of the cluster
+    __shared__ volatile int s_parts, s_rows;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
@@ -324,7 +334,12 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     if (warp < 4) {
         const int row = tid, token = row * inverse >> 16, head = g * p.ratio + row - token * p.ratio;
         const bool on = token < used;
-        const int m = first + t0 + token, last = on ? len + t0 + token - skip * kKT : -1;         // the row's place in the buffers, its newest key
+        const int m = first + t0 + token;
+        const int last = on ? len + t0 + token - skip * kKT : -1;         // the row's place in the buffers, its newest key
+        s_out[row] = on ? p.out + (size_t)m * p.ldo + head * HD : nullptr;
+        s_stat[row] = on && p.stats != nullptr && t0 + token >= room - p.window ? m * p.H + head : -1;
+        s_since[row] = 1.0f;
+        if (row == 0) { s_parts = parts; s_rows = used * p.ratio; }          // the arrival for the queries publishes them
         float c = 1.0f, top = -INFINITY;
         float2 sums = make_float2(0.0f, 0.0f);
         if (tiles > 0) {
@@ -335,11 +350,48 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         }
         const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
         bool ok = true;
+        // Totals of this warp's rows, in the rows of the output or (blocks of a cluster) the workspace: float4s i of all rows are side by side.
+        auto total = [&](int i, int there, bool shared) {
+            const int at = i * there + lane, r = warp * 32 + at / (HD / 4);
+            return (shared ? p.totals + ((size_t)blockIdx.x * kPT + r) * HD : s_out[r]) + 4 * (at % (HD / 4));
+        };
+        auto add_to_totals = [&](bool fresh) {
+            const float since = s_since[tid];
+            const bool plain = !fresh && __all_sync(0xffffffffu, since == 1.0f);
+            const int there = min(32, s_rows - warp * 32);
+            const bool shared = s_parts > 1;
+#pragma unroll 1
+            for (int k = 0; k < HD; k += 32) {
+                uint32_t o[32];
+                tmem_ld32(mine + kO + k, o);
+                if (lane < there)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float* const at = total(k / 4 + i, there, shared);
+                        float4 v = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                        if (plain) {
+                            asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+                        } else {
+                            if (!fresh) {
+                                const float4 w = __ldcg(reinterpret_cast<const float4*>(at));
+                                v.x = fmaf(w.x, since, v.x); v.y = fmaf(w.y, since, v.y); v.z = fmaf(w.z, since, v.z); v.w = fmaf(w.w, since, v.w);
+                            }
+                            __stcg(reinterpret_cast<float4*>(at), v);
+                        }
+                    }
+            }
+            s_since[tid] = 1.0f;
+        };
 #pragma unroll 1
         for (int j = 0; j < tiles; j++) {
             if (!__all_sync(0xffffffffu, mbar_wait_long(sFull(j & 1), (j >> 1) & 1, &s_abort, p.error, 341))) ok = false;
             tc_fence_after();
             const uint32_t at = mine + (uint32_t)((j & 1) * kKT);
+            if (j > 0 && j % kSegment == 0) {                            // the next product starts from zero
+                if (!__all_sync(0xffffffffu, mbar_wait_long(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
+                tc_fence_after();
+                add_to_totals(j == kSegment);
+            }
             const int left = last - j * kKT;                             // newest key within the tile
             const bool cut = !__all_sync(0xffffffffu, left >= kKT - 1);
             float most = -INFINITY;
@@ -364,7 +416,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             const bool grown = most > top + 8.0f;                        // also the first keys of a row
             if (__any_sync(0xffffffffu, grown)) {
                 const float now = grown ? most : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
-                if (j > 0) {
+                if (j % kSegment > 0) {
                     if (!__all_sync(0xffffffffu, mbar_wait_long(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
                     tc_fence_after();
 #pragma unroll 1
@@ -377,6 +429,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                     }
                 }
                 sums.x *= f; sums.y *= f;
+                s_since[tid] *= f;
                 top = now;
             }
             const float shift = top > -INFINITY ? -top : 0.0f;           // a row without keys yet: every weight is 2^-inf
@@ -407,13 +460,25 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
             ok = __all_sync(0xffffffffu, ok && mbar_wait_long(done, 0, &s_abort, p.error, 343));
             tc_fence_after();
-            const float sum = sums.x + sums.y, inv = parts > 1 ? 1.0f : 1.0f / sum;
-            if (parts > 1) s_row[row] = make_float2(top, sum);
             float* const stage = reinterpret_cast<float*>(smem);
+            const float since = s_since[tid];
+            const int there = min(32, s_rows - warp * 32);
+            const bool shared = s_parts > 1;
+            const float sum = sums.x + sums.y, inv = shared ? 1.0f : 1.0f / sum;
+            if (shared) s_row[row] = make_float2(top, sum);
 #pragma unroll 1
             for (int k = 0; ok && k < HD; k += 32) {
                 uint32_t o[32];
                 tmem_ld32(mine + kO + k, o);
+                if (tiles > kSegment && lane < there)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 w = __ldcg(reinterpret_cast<const float4*>(total(k / 4 + i, there, shared)));
+                        o[4 * i] = __float_as_uint(fmaf(w.x, since, __uint_as_float(o[4 * i])));
+                        o[4 * i + 1] = __float_as_uint(fmaf(w.y, since, __uint_as_float(o[4 * i + 1])));
+                        o[4 * i + 2] = __float_as_uint(fmaf(w.z, since, __uint_as_float(o[4 * i + 2])));
+                        o[4 * i + 3] = __float_as_uint(fmaf(w.w, since, __uint_as_float(o[4 * i + 3])));
+                    }
 #pragma unroll
                 for (int i = 0; i < 8; i++) {     // dims 4t … 4t + 3, 16 dims on for the high nibbles
                     const int from = 8 * (i & 3) + 2 * (i >> 2);
@@ -422,15 +487,13 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 }
             }
             __syncwarp();                         // a warp stores the rows that it has staged
-            const int rows = parts > 1 ? 0 : min(32, used * p.ratio - warp * 32), e = lane % LPR;
+            const int e = lane % LPR;
+            if (ok && !shared) {
 #pragma unroll 8
-            for (int i = lane / LPR; i < rows; i += RPW) {
-                const int r = warp * 32 + i, t = r * inverse >> 16;
-                const float4 v = *reinterpret_cast<const float4*>(stage + r * PITCH + 4 * e);
-                if (ok) *reinterpret_cast<float4*>(p.out + (size_t)(first + t0 + t) * p.ldo + (g * p.ratio + r - t * p.ratio) * HD + 4 * e) = v;
+                for (int i = lane / LPR; i < there; i += RPW)
+                    *reinterpret_cast<float4*>(s_out[warp * 32 + i] + 4 * e) = *reinterpret_cast<const float4*>(stage + (warp * 32 + i) * PITCH + 4 * e);
+                if (s_stat[row] >= 0) *reinterpret_cast<float2*>(p.stats + (size_t)s_stat[row] * 2) = make_float2(top, sum);
             }
-            if (parts == 1 && on && p.stats != nullptr && t0 + token >= room - p.window)
-                *reinterpret_cast<float2*>(p.stats + ((size_t)m * p.H + head) * 2) = make_float2(top, sum);
         }
     } else if (warp < 12) {
         const bool value = warp >= 8;
@@ -483,7 +546,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int c = 0; c < S::kChunks; c++) {
-                    const uint64_t a = q0 + (uint32_t)((h * S::kQ + c * (kPT * 128)) >> 4), b = k0 + (uint32_t)((c * (kKT * 128)) >> 4);
+                    const uint64_t a = q0 + (uint32_t)(((1 - h) * S::kQ + c * (kPT * 128)) >> 4), b = k0 + (uint32_t)((c * (kKT * 128)) >> 4);
 #pragma unroll
                     for (int k = 0; k < (HD < 64 ? HD / 16 : 4); k++) umma_f16_by(lead, d, a + 2 * k, b + 2 * k, kIdescQK, (h | c | k) != 0);
                 }
@@ -508,7 +571,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 const uint32_t a = tmem + (uint32_t)((j & 1) * kKT);
 #pragma unroll
                 for (int k = 0; k < kKT / 16; k++) {
-                    umma_f16_ta_by(lead, tmem + kO, a + (k >> 1) * 32 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, (j | k) != 0);
+                    umma_f16_ta_by(lead, tmem + kO, a + (k >> 1) * 32 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, (j % kSegment | k) != 0);
                     umma_f16_ta_by(lead, tmem + kO, a + (k >> 1) * 32 + 16 + (k & 1) * 8, v0 + (uint32_t)(k * 2048 >> 4), kIdescPV, 1);
                 }
                 umma_commit_by(lead, vEmpty);
@@ -521,9 +584,10 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         // every block of the cluster joins a part of the rows: Σ 2^(mᵢ − m)·Oᵢ over the sum of the same with the sums of weights
         __syncwarp();
         cluster_sync();
+        const int parts = s_parts, all = s_rows, rank = blockIdx.x % p.splits;
         if (parts > 1 && rank < parts && !s_abort) {
             const uint32_t stage = base, state = smem_u32(s_row);
-            const int all = used * p.ratio, r1 = all * (rank + 1) / parts, e = lane % LPR;
+            const int r1 = all * (rank + 1) / parts, e = lane % LPR;
 #pragma unroll 2
             for (int r = all * rank / parts + warp * RPW + lane / LPR; r < r1; r += (kPThreads / 32) * RPW) {
                 float2 of[kMaxSplits];
@@ -548,10 +612,8 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                     v.x = fmaf(o[i].x, f, v.x); v.y = fmaf(o[i].y, f, v.y); v.z = fmaf(o[i].z, f, v.z); v.w = fmaf(o[i].w, f, v.w);
                 }
                 const float inv = 1.0f / sum;
-                const int t = r * inverse >> 16, head = g * p.ratio + r - t * p.ratio;
-                const size_t m = first + t0 + t;
-                *reinterpret_cast<float4*>(p.out + m * p.ldo + head * HD + 4 * e) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                if (e == 0 && p.stats != nullptr && t0 + t >= room - p.window) *reinterpret_cast<float2*>(p.stats + (m * p.H + head) * 2) = make_float2(top, sum);
+                *reinterpret_cast<float4*>(s_out[r] + 4 * e) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                if (e == 0 && s_stat[r] >= 0) *reinterpret_cast<float2*>(p.stats + (size_t)s_stat[r] * 2) = make_float2(top, sum);
             }
         }
         __syncwarp();
@@ -648,7 +710,7 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
 #pragma unroll
                         for (int k = 0; k < HD / 16; k++) {
                             const uint32_t o = (uint32_t)((k >> 2) * (kPT * 128) + (k & 3) * 32);
-                            umma_f16(tmem, desc_k(base + 2 * S::kTile + o), desc_k(base + h * S::kTile + o), kIdesc, (h | k) != 0);
+                            umma_f16(tmem, desc_k(base + 2 * S::kTile + o), desc_k(base + (1 - h) * S::kTile + o), kIdesc, (h | k) != 0);
                         }
                     umma_commit(smem_u32(&s_bar));
                 }
@@ -694,31 +756,40 @@ long long resident(int n) {
     return most[n];
 }
 
+struct Plan { long long blocks; int splits, least; bool alone; };
+// Few blocks share their keys in clusters, as far as all are resident: a block takes 0.97 µs for a tile (64 values a row) with an SM to itself, two on
+// one 1.48.  A second wave costs more than it gives (96 blocks of 300 queries before 3300 keys: 82 µs alone, 64 by twos, 69 by threes, of which 90 fit).
+// Joining takes some 3 µs: four tiles to a block at least, five where two are on an SM (512 queries of 32 heads × 128: 37 µs, with fours 41).
 template <int NB>
-void prefill(const PrefillParams& p, cudaStream_t s) {
+Plan plan_of(const Q4AttnArgs& a) {
     static bool attr = false;
     if (!attr) {
         DJ_CUDA_CHECK(cudaFuncSetAttribute(k_q4_prefill<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAlone));
         DJ_CUDA_CHECK(cudaFuncSetAttribute(k_q4_window<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)WindowShape<NB>::kSmem));
         attr = true;
     }
-    const int per = kPT / p.ratio;                // tokens of a tile; a sequence has at most one that is not full
-    const long long blocks = (long long)p.G * ((p.M + per - 1) / per + std::min(p.B, p.M) - 1);
-    PrefillParams q = p;
-    // Few blocks share their keys in clusters, as far as all are resident: a block takes 0.97 µs for a tile (64 values a row) with an SM to itself, two on
-    // one 1.48.  A second wave costs more than it gives (96 blocks of 300 queries before 3300 keys: 82 µs alone, 64 by twos, 69 by threes, of which 90 fit).
-    // Joining takes some 3 µs: four tiles to a block at least, five where two are on an SM (512 queries of 32 heads × 128: 37 µs, with fours 41).
-    bool alone = blocks <= g_num_sms;
-    double best = alone ? 1.0 : 1.5;
+    const int per = kPT / (a.H / a.G);            // tokens of a tile; a sequence has at most one that is not full
+    Plan plan = {(long long)a.G * ((a.M + per - 1) / per + std::min(a.B, a.M) - 1), 1, 1, false};
+    plan.alone = plan.blocks <= g_num_sms;
+    double best = plan.alone ? 1.0 : 1.5;
     for (int n = 2; n <= kMaxSplits; n++)
         for (int two = 0; two < 2; two++) {
-            const int least = two ? 5 : 4, parts = std::min(n, p.maxSeq / (least * kKT));
-            const double cost = (two ? 1.5 : 1.0) / parts;
-            if (parts > 1 && cost < best && blocks <= (two + 1) * resident<NB>(n)) { best = cost; alone = !two; q.splits = n; q.least = least; }
+            const int least = two ? 5 : 4, parts = std::min(n, a.maxSeq / (least * kKT));
+            const double cost = (two ? 1.5 : 1.0) / std::max(parts, 1);
+            if (parts > 1 && cost < best && plan.blocks <= (two + 1) * resident<NB>(n)) { best = cost; plan.alone = !two; plan.splits = n; plan.least = least; }
         }
+    return plan;
+}
+Plan plan_of(const Q4AttnArgs& a) { return a.hd == 128 ? plan_of<4>(a) : a.hd == 64 ? plan_of<2>(a) : plan_of<1>(a); }
+
+size_t stats_floats(const Q4AttnArgs& a) { return a.accOut != nullptr ? ((size_t)a.M * a.H * 2 + 3) / 4 * 4 : 0; }
+
+template <int NB>
+void prefill(PrefillParams p, const Plan& plan, cudaStream_t s) {
+    p.splits = plan.splits; p.least = plan.least;
     // a grid that gives every block an SM of its own asks for so much shared memory that it gets one (blocks are dealt out two to an SM otherwise)
-    const size_t smem = alone ? kAlone : PrefillShape<NB>::kSmem;
-    if (p.M > 0) launch_k_cluster(k_q4_prefill<NB>, dim3((unsigned)(blocks * q.splits)), dim3(kPThreads), smem, s, dim3(q.splits), q);
+    const size_t smem = plan.alone ? kAlone : PrefillShape<NB>::kSmem;
+    if (p.M > 0) launch_k_cluster(k_q4_prefill<NB>, dim3((unsigned)(plan.blocks * p.splits)), dim3(kPThreads), smem, s, dim3(p.splits), p);
     // a block's queries serve all its key tiles: about two blocks per SM
     const int tiles = (p.maxSeq + kPT - 1) / kPT, share = std::max(1, 2 * g_num_sms / std::max(1, p.G * p.B));
     if (p.accOut != nullptr) launch_k(k_q4_window<NB>, dim3(std::min(tiles, share), p.G, p.B), dim3(kWThreads), WindowShape<NB>::kSmem, s, true, p);
@@ -726,14 +797,18 @@ void prefill(const PrefillParams& p, cudaStream_t s) {
 
 }  // namespace
 
-size_t q4_attn_ws_floats(const Q4AttnArgs& a) { return a.accOut != nullptr ? (size_t)a.M * a.H * 2 : 0; }
+size_t q4_attn_ws_floats(const Q4AttnArgs& a) {
+    const Plan plan = plan_of(a);
+    return stats_floats(a) + (a.M > 0 && plan.splits > 1 && a.maxSeq > kSegment * kKT ? (size_t)plan.blocks * plan.splits * kPT * a.hd : 0);
+}
 
 void launch_q4_attn(const Q4AttnArgs& a, cudaStream_t s) {
-    PrefillParams p = {a.qkv, a.q_off, a.ld, a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.starts, a.len, a.pos, a.cosT, a.sinT, a.maxPos, a.out, a.ldo,
-                       a.B, a.H, a.G, a.H / a.G, a.M, (float)(1.0 / std::sqrt((double)a.hd) * 1.4426950408889634), a.accOut != nullptr ? a.ws : nullptr, a.window,
-                       a.acc, a.accOut, g_dev_error, 1, 1};
+    const PrefillParams p = {a.qkv, a.q_off, a.ld, a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.starts, a.len, a.pos, a.cosT, a.sinT, a.maxPos, a.out, a.ldo,
+                             a.B, a.H, a.G, a.H / a.G, a.M, (float)(1.0 / std::sqrt((double)a.hd) * 1.4426950408889634), a.accOut != nullptr ? a.ws : nullptr, a.window,
+                             a.acc, a.accOut, g_dev_error, a.ws + stats_floats(a), 1, 1};
+    const Plan plan = plan_of(a);
     if (a.M > 0) launch_q4_append(a, 1, s);
-    if (a.hd == 128) prefill<4>(p, s); else if (a.hd == 64) prefill<2>(p, s); else prefill<1>(p, s);
+    if (a.hd == 128) prefill<4>(p, plan, s); else if (a.hd == 64) prefill<2>(p, plan, s); else prefill<1>(p, plan, s);
 }
 
 }  // namespace dj

@@ -763,6 +763,7 @@ void do_op(Ctx& ctx, const int32_t* c) {
             a.len = f32(ctx, e[8], a.B, what); a.pos = f32(ctx, e[9], a.B, what);
             a.cosT = f32(ctx, e[10], sz(a.maxPos, a.hd / 2), what); a.sinT = f32(ctx, e[11], sz(a.maxPos, a.hd / 2), what);
             a.out = f32(ctx, e[13], a.M ? (size_t)e[14] + sz(last, a.ldo) + a.H * a.hd : 0, what) + e[14];
+            require(a.M == 0 || e[13] != c[1], what, "the output goes to another buffer than the rows");
             require((w[0] < 0) == (w[1] < 0), what, "accumulated weights need both an input and an output (which may be the same buffer)");
             require(!packed || (w[0] < 0) == (a.window == 0), what, "a window goes with accumulated weights, and they with a window");
             a.acc = f32_opt(ctx, w[0], sz(a.B, a.G) * a.maxSeq, what); a.accOut = f32_opt(ctx, w[1], sz(a.B, a.G) * a.maxSeq, what);
