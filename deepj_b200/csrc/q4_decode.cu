@@ -191,6 +191,7 @@ struct DecodeWarp {
             q4_put_row<NB>(cached, r, false, e, kx, lane < LPR);
             q4_put_row<NB>(cached, r, true, e, vx, lane < LPR);
         }
+        fence_proxy_async_smem();                 // a copy will come over the page
         __syncwarp();
     }
 

@@ -217,6 +217,10 @@ __device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
 }
 __device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 
+// what a block that gives up still has on its way
+__device__ __forceinline__ void wait_out(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < 1 << 16 && !mbar_try_wait(bar, parity); i++) {}
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -512,8 +516,9 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         };
         request(0);
         if (tiles > 0) queries();
+        int j = 0, asked = 0;                     // asked: the last tile whose rows were
 #pragma unroll 1
-        for (int j = 0; j < tiles; j++) {
+        for (; j < tiles; j++) {
             const bool there = 2 * j + (w >> 1) < pages;
             uint32_t words[2][NB];
             float scale[NB];
@@ -525,7 +530,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 for (int i = 0; i < NB; i++)
                     scale[i] = __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(raw_at + 16 * Q4Page<NB>::kRow + ((lane & 15) * NB + i) * 2) << 16);
                 __syncwarp();
-                request(j + 1);                   // everything of this tile is in registers
+                request(asked = j + 1);           // everything of this tile is in registers
             }
             if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait_long(value ? vEmpty : kEmpty, (j - 1) & 1, &s_abort, p.error, 344))) break;
             if (there) convert_pieces<NB, kKT>(words, scale, tile, row, t0w);
@@ -534,6 +539,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             __syncwarp();
             if (lane == 0) mbar_arrive(value ? vFull : kFull);
         }
+        if (j < tiles && 2 * min(asked, tiles - 1) + (w >> 1) < pages) wait_out(arrived, min(asked, tiles - 1) & 1);
     } else {
         // The whole warp walks the loop and one lane's predicate issues: in one lane's branch every operand would be moved into a uniform register first (70
         // cycles an MMA).  Rolled: what is issued has to come from the instruction cache in time.
@@ -556,8 +562,9 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         if (tiles > 0 && waited(qReady, 0, 349) && waited(kFull, 0, 346)) {
             tc_fence_after();
             scores(0);
+            int j = 0;
 #pragma unroll 1
-            for (int j = 0; j < tiles; j++) {
+            for (; j < tiles; j++) {
                 if (j + 1 < tiles) {
                     // P·V of tile j - 1 has read the buffer that the scores of j + 1 go to
                     if (j >= 1 && !waited(vEmpty, (j - 1) & 1, 350)) break;
@@ -577,6 +584,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 umma_commit_by(lead, vEmpty);
             }
             umma_commit_by(lead, done);
+            if (j < tiles) wait_out(done, 0);
         }
         __syncwarp();
     }
