@@ -10,12 +10,13 @@ namespace {
 
 // ───────────── rows in ─────────────
 // Row m of the source is token t of sequence b: m = b·T + t, or (starts) the packed row that lies in starts[b] … starts[b + 1].  A row of a head is
-// 8·NB lanes of four values.  Bound by the bytes: 8·hd read and 1.125·hd written per row and head.
+// 4·NB lanes of eight values, a word of the page each.  The bytes are 8·hd read and 1.125·hd written per row and head; what bounds it is the instructions
+// for the codes (2048 rows of 32 heads of 128: 20 µs where the bytes take 12; with four values to a lane 27).
 struct AppendParams {
     const float* src; int k_off, v_off, ld;
     unsigned char* cache; int maxSeq, pages;
     const float* starts; const float* len; const float* pos; const float* cosT; const float* sinT; int maxPos;
-    int B, G, T, M, share;                               // share: warps of a row (a power of two up to eight)
+    int B, G, T, M, share;                               // share: warps of a row (a power of two)
 };
 
 // The sequence that packed row m belongs to (the first, should ranges overlap), or -1; whole warps call it.
@@ -37,7 +38,7 @@ __device__ __forceinline__ int sequence_of(const float* starts, int B, int M, in
 
 template <int NB>
 __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
-    constexpr int LPR = 8 * NB, RPW = 32 / LPR;          // lanes of a row, rows of a warp
+    constexpr int LPR = 4 * NB, RPW = 32 / LPR;          // lanes of a row, rows of a warp
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, at = blockIdx.x * 8 + (threadIdx.x >> 5), m = at / p.share, part = at - m * p.share;
@@ -52,31 +53,40 @@ __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
     }
     const int t = m - first, len = (int)p.len[b], pos = p.pos != nullptr ? (int)p.pos[b] : 0;
     if (t >= q4_room(tokens, len, p.maxSeq, pos, p.pos != nullptr ? p.maxPos : 0x7fffffff)) return;
-    const int row = len + t, e = lane % LPR;
+    const int row = len + t, f = lane % LPR, at0 = (f >> 2) * 32 + (f & 3) * 4;      // this lane's values: at0 … at0 + 3, and 16 on
     const float* src = p.src + (size_t)m * p.ld;
-    float2 c = make_float2(1.0f, 1.0f), s = make_float2(0.0f, 0.0f);
-    if (p.cosT != nullptr) {
-        const size_t at = (size_t)(pos + t) * (16 * NB) + 2 * e;
-        c = *reinterpret_cast<const float2*>(p.cosT + at); s = *reinterpret_cast<const float2*>(p.sinT + at);
-    }
+    float2 c[2] = {{1.0f, 1.0f}, {1.0f, 1.0f}}, s[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+    if (p.cosT != nullptr)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const size_t at = (size_t)(pos + t) * (16 * NB) + (at0 >> 1) + 8 * h;
+            c[h] = *reinterpret_cast<const float2*>(p.cosT + at); s[h] = *reinterpret_cast<const float2*>(p.sinT + at);
+        }
     // keys of all heads, then their values, four rows of a warp at a time: their loads go out together
     constexpr int kAhead = 4;
+    const size_t plane = (size_t)p.pages * Q4Page<NB>::kBytes;
+    unsigned char* const pages = p.cache + (size_t)b * p.G * plane + (size_t)(row / kQ4Page) * Q4Page<NB>::kBytes;
+    const int in = row % kQ4Page;
 #pragma unroll 1
     for (int i0 = part * RPW; i0 < 2 * p.G; i0 += p.share * RPW * kAhead) {
-        float4 x[kAhead];
+        float4 x[kAhead][2];
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
             const int i = i0 + k * p.share * RPW + lane / LPR;
-            x[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i < 2 * p.G) x[k] = *reinterpret_cast<const float4*>(src + (i < p.G ? p.k_off + i * (32 * NB) : p.v_off + (i - p.G) * (32 * NB)) + 4 * e);
+            x[k][0] = x[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < 2 * p.G) {
+                const float* const from = src + (i < p.G ? p.k_off + i * (32 * NB) : p.v_off + (i - p.G) * (32 * NB)) + at0;
+                x[k][0] = *reinterpret_cast<const float4*>(from); x[k][1] = *reinterpret_cast<const float4*>(from + 16);
+            }
         }
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
             if (i0 + k * p.share * RPW >= 2 * p.G) break;
             const int i = i0 + k * p.share * RPW + lane / LPR, g = i < p.G ? i : i - p.G;
-            if (i < p.G && p.cosT != nullptr) x[k] = q4_rotate(x[k], c, s);
-            unsigned char* page = p.cache + (((size_t)b * p.G + g) * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
-            q4_put_row<NB>(page, row % kQ4Page, i >= p.G, e, x[k], i < 2 * p.G);
+            if (i < p.G && p.cosT != nullptr)
+#pragma unroll
+                for (int h = 0; h < 2; h++) x[k][h] = q4_rotate(x[k][h], c[h], s[h]);
+            q4_put_words<NB>(pages + g * plane, in, i >= p.G, f, x[k][0], x[k][1], i < 2 * p.G);
         }
     }
 }
@@ -294,8 +304,9 @@ size_t q4_plane_bytes(int B, int G, int maxSeq, int hd) { return (size_t)B * G *
 
 void launch_q4_append(const Q4AttnArgs& a, int T, cudaStream_t s) {
     AppendParams p = {a.qkv, a.k_off, a.v_off, a.ld, a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.starts, a.len, a.pos, a.cosT, a.sinT, a.maxPos, a.B, a.G, T, a.M, 1};
-    // few rows are shared by warps; with one warp to a row the place of a row is looked up once and its heads' loads follow one another
-    while (p.share < 8 && (long long)a.M * p.share < 24 * g_num_sms) p.share *= 2;
+    // A warp takes some sixteen keys and values of a row, so that its place is looked up seldom (8848 rows of 8 heads of 128: 27 µs with one warp to a row,
+    // 31 with four; 2048 of 32 heads: 29 with one, 26 with four); fewer where there are few rows (16 of 32 heads: 25.6 with one, 12 with sixteen).
+    while (p.share < 16 && (p.G / p.share >= 16 || (long long)a.M * p.share < 24 * g_num_sms)) p.share *= 2;
     if (a.hd == 128) append<4>(p, s); else if (a.hd == 64) append<2>(p, s); else append<1>(p, s);
 }
 void launch_q4_load(const Q4LoadArgs& a, cudaStream_t s) {

@@ -32,45 +32,64 @@ __device__ __forceinline__ int q4_room(int tokens, int len, int maxSeq, int pos,
     return max(0, min(tokens, min(maxSeq - len, maxPos - pos)));
 }
 
-// The eight lanes of a block hold four values each → the block's scale and this lane's four codes in the low nibbles of a word's bytes.  The code is the
-// rounded quotient; a product with the reciprocal is within 2e-6 of it, so only values that close to the middle of two codes need the division (2048
-// rows of 64 × 128, with the rotation: 33 µs dividing all).
-__device__ __forceinline__ uint32_t q4_codes(const float4& x, float& scale) {
-    float most = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));           // of the values that are no NaN
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    most = most == most ? most : 0.0f;
-    const float s = fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(most * (1.0f / 7.0f))), kQ4ScaleMin), kQ4ScaleMax), inverse = __frcp_rn(s);
-    scale = most > 0.0f ? s : 0.0f;
-    // the sum with 1.5 · 2^23 ends in the rounded quotient, in two's complement
-    uint32_t codes = 0;
-    float off = 0.0f;                             // the largest distance from a whole number
+// The scale of a block whose largest magnitude is `most` (of the values that are no NaN).
+__device__ __forceinline__ float q4_scale(float most) { return fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(most * (1.0f / 7.0f))), kQ4ScaleMin), kQ4ScaleMax); }
+__device__ __forceinline__ float q4_most(const float4& x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); }
+// Four values' codes in the low nibbles of a word's bytes.  The code is the rounded quotient; a product with the reciprocal is within 2e-6 of it, so only
+// values that close to the middle of two codes need the division (2048 rows of 64 × 128, with the rotation: 33 µs dividing all).  The sum with 1.5 · 2^23
+// ends in the rounded quotient, in two's complement.  off: raised to the largest distance from a whole number.
+__device__ __forceinline__ uint32_t q4_near(const float4& x, float inverse, float& off) {
     const float v[4] = {x.x, x.y, x.z, x.w};
+    uint32_t codes = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float q = v[i] * inverse, sum = q + 12582912.0f;
         off = fmaxf(off, fabsf(q - (sum - 12582912.0f)));
         codes |= ((uint32_t)__float_as_int(sum) & 15u) << (8 * i);
     }
-    // blocks that saturate, NaN and infinities take this way too
-    const float all = (v[0] + v[1]) + (v[2] + v[3]);
-    if (__any_sync(0xffffffffu, off > 0.4999f || most > 7.0f * kQ4ScaleMax || all != all)) {
-        codes = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) codes |= ((uint32_t)min(max(__float2int_rn(v[i] / s), -7), 7) & 15u) << (8 * i);      // NaN → 0
-    }
     return codes;
+}
+__device__ __forceinline__ uint32_t q4_divided(const float4& x, float s) {
+    auto code = [](float v) { return (uint32_t)min(max(__float2int_rn(v), -7), 7) & 15u; };     // NaN → 0
+    return code(x.x / s) | code(x.y / s) << 8 | code(x.z / s) << 16 | code(x.w / s) << 24;
 }
 
 // 8·NB consecutive lanes (all lanes of the warp are here) put one row into its page: lane e of them holds the values 4e … 4e + 3.
 template <int NB>
 __device__ __forceinline__ void q4_put_row(unsigned char* page, int row, bool value, int e, const float4& x, bool on) {
-    float scale;
-    const uint32_t mine = q4_codes(x, scale), other = __shfl_xor_sync(0xffffffffu, mine, 4);
+    float most = q4_most(x);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = most == most ? most : 0.0f;
+    const float s = q4_scale(most);
+    float off = 0.0f;
+    uint32_t mine = q4_near(x, __frcp_rn(s), off);
+    const float all = (x.x + x.y) + (x.z + x.w);  // blocks that saturate, NaN and infinities are divided too
+    if (__any_sync(0xffffffffu, off > 0.4999f || most > 7.0f * kQ4ScaleMax || all != all)) mine = q4_divided(x, s);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 4);
     if (!on) return;
     const int j = e >> 3, t = e & 3;
     if ((e & 4) == 0) *reinterpret_cast<uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(row, t, j)) = mine | other << 4;
-    if ((e & 7) == 0) *reinterpret_cast<__nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (row * NB + j) * 2) = __float2bfloat16_rn(scale);
+    if ((e & 7) == 0) *reinterpret_cast<__nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (row * NB + j) * 2) = __float2bfloat16_rn(most > 0.0f ? s : 0.0f);
+}
+// 4·NB lanes: lane f holds the values 32j + 4t … + 3 (x) and 16 values on (y), j = f / 4, t = f % 4: a word of the page.
+template <int NB>
+__device__ __forceinline__ void q4_put_words(unsigned char* page, int row, bool value, int f, const float4& x, const float4& y, bool on) {
+    float most = fmaxf(q4_most(x), q4_most(y));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = most == most ? most : 0.0f;
+    const float s = q4_scale(most), inverse = __frcp_rn(s);
+    float off = 0.0f;
+    uint32_t word = q4_near(x, inverse, off);
+    word |= q4_near(y, inverse, off) << 4;
+    const float all = ((x.x + x.y) + (x.z + x.w)) + ((y.x + y.y) + (y.z + y.w));
+    if (__any_sync(0xffffffffu, off > 0.4999f || most > 7.0f * kQ4ScaleMax || all != all)) word = q4_divided(x, s) | q4_divided(y, s) << 4;
+    if (!on) return;
+    const int j = f >> 2, t = f & 3;
+    unsigned char* const half = page + (value ? Q4Page<NB>::kV : 0);
+    *reinterpret_cast<uint32_t*>(half + Q4Page<NB>::word(row, t, j)) = word;
+    if (t == 0) *reinterpret_cast<__nv_bfloat16*>(half + Q4Page<NB>::kKs + (row * NB + j) * 2) = __float2bfloat16_rn(most > 0.0f ? s : 0.0f);
 }
 
 // interleaved pairs (x0, x1) → (x0·c − x1·s, x0·s + x1·c), every product and sum rounded (RotaryEmbedding.java:81-122)
