@@ -153,23 +153,23 @@ __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, i
 }
 
 // Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 8·NB lanes of four values each; `place(row, m, head, position)` says
-// which one row `row` is, and whether it is one (false: zeros, but the place can be read).  factors[row] makes a sum of products a score in log2 units
+// which one row `row` of the first `rows` is, and whether it is one (false: zeros, but the place can be read).  factors[row] makes a sum of products a score in log2 units
 // (NaN where the row holds an infinity or a NaN).  Four rows' loads go out together: one after another they took 20000 cycles a tile.
 template <int NB, typename Place>
-__device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, Place place) {
+__device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, int rows, Place place) {
     constexpr int HD = 32 * NB, LPR = 8 * NB, RPW = 32 / LPR, AHEAD = 4;
     const int e = lane % LPR;
     // this lane's dims 4e … 4e + 3 in the tiles' order: (0, 2) and (1, 3), eight bytes apart
     const int piece = (e >> 3) * 4 + (e & 3), at = (piece >> 3) * (kPT * 128) + (e & 4);
 #pragma unroll 1
-    for (int r0 = warp * RPW + lane / LPR; r0 < kPT; r0 += AHEAD * warps * RPW) {
+    for (int r0 = warp * RPW + lane / LPR; r0 < rows; r0 += AHEAD * warps * RPW) {
         float4 x[AHEAD];
         float2 cs[AHEAD], sn[AHEAD];
         bool on[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             int m, head, position;
-            on[k] = place(min(r0 + k * warps * RPW, kPT - 1), m, head, position);
+            on[k] = place(min(r0 + k * warps * RPW, rows - 1), m, head, position);
             const size_t tab = (size_t)position * (HD / 2) + 2 * e;
             x[k] = *reinterpret_cast<const float4*>(p.qkv + (size_t)m * p.ld + p.q_off + head * HD + 4 * e);
             cs[k] = *reinterpret_cast<const float2*>(p.cosT + tab);
@@ -193,11 +193,12 @@ __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int
             uint2 h, l;
             split_half(y.x * mul, y.z * mul, h.x, l.x);
             split_half(y.y * mul, y.w * mul, h.y, l.y);
-            if (r >= kPT) break;
-            const int to = at + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-            *reinterpret_cast<uint32_t*>(hi + to) = h.x; *reinterpret_cast<uint32_t*>(hi + to + 8) = h.y;
-            *reinterpret_cast<uint32_t*>(lo + to) = l.x; *reinterpret_cast<uint32_t*>(lo + to + 8) = l.y;
-            if (e == 0) factors[r] = fine ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
+            if (r < rows) {
+                const int to = at + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint32_t*>(hi + to) = h.x; *reinterpret_cast<uint32_t*>(hi + to + 8) = h.y;
+                *reinterpret_cast<uint32_t*>(lo + to) = l.x; *reinterpret_cast<uint32_t*>(lo + to + 8) = l.y;
+                if (e == 0) factors[r] = fine ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
+            }
         }
     }
 }
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
 
     const int inverse = 65535 / p.ratio + 1;      // r · inverse / 2^16 is r / ratio for a row r of the tile
     auto queries = [&]() {                        // twelve warps lay the queries down
-        query_rows<NB>(p, warp, 12, lane, smem, smem + S::kQ, s_factor, [&](int r, int& qm, int& qh, int& qp) {
+        query_rows<NB>(p, warp, 12, lane, smem, smem + S::kQ, s_factor, kPT, [&](int r, int& qm, int& qh, int& qp) {
             const int t = min(r * inverse >> 16, used - 1);
             qm = first + t0 + t; qh = g * p.ratio + min(r - t * p.ratio, p.ratio - 1); qp = pos + t0 + t;
             return r < used * p.ratio;
@@ -634,25 +635,25 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
 
 // ───────────── weights of the last tokens ─────────────
 // Row i of a key/value head: its old weight and the softmax weights of the sequence's last `window` tokens.  The product is taken the other way round,
-// Sᵀ = K·Qᵀ, so that a thread is a key and adds up its row over the queries in a fixed order.  A block takes 128 keys and 128 query rows at a time.
-constexpr int kWThreads = 128;
+// Sᵀ = K·Qᵀ, so that a thread is a key and half of the queries and adds up its row over them in a fixed order.  A block takes 128 keys and 128 query rows
+// at a time.  Bound by latency: laying the queries down, one tile after the other.
+constexpr int kWThreads = 256;
 template <int NB> struct WindowShape {
     static constexpr int kTile = PrefillShape<NB>::kQ;
     static constexpr int kHalvesAt = 3 * kTile;                          // Q hi, Q lo, K
     static constexpr size_t kSmem = (size_t)kHalvesAt + 4 * Q4Page<NB>::kHalf + 1024;
 };
 template <int NB>
-__global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) {
+__global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams p) {
     using S = WindowShape<NB>;
     constexpr int HD = 32 * NB;
-    constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kPT >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long s_bar;
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
-    __shared__ float s_factor[kPT];
+    __shared__ float s_factor[kPT], s_half[kPT];  // s_half: the sums of the second half of the queries
     __shared__ float4 s_row[kPT];                 // factor, maximum, 1 / sum, newest key of every query row
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mine = tid & (kPT - 1), part = tid / kPT, g = blockIdx.y, b = blockIdx.z;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
     if (tid == 0) {
@@ -672,64 +673,68 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
     const int room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos), keys = there ? len + room : 0, pages = (keys + kQ4Page - 1) / kQ4Page;
     const int window = min(p.window, room), rows = window * p.ratio;
     const uint32_t tmem = s_tmem;
-    unsigned char* const half = smem + S::kHalvesAt + warp * Q4Page<NB>::kHalf;
+    unsigned char* const half = smem + S::kHalvesAt + (warp & 3) * Q4Page<NB>::kHalf;
     const unsigned char* const plane = p.cache + ((size_t)b * p.G + g) * p.pages * Q4Page<NB>::kBytes;
-    auto fetch = [&](int k0) {                    // this warp's page of a tile
-        const int pg = k0 / kQ4Page + warp;
+    auto fetch = [&](int k0) {                    // a page of a tile to two warps
+        const int pg = k0 / kQ4Page + (warp & 3);
         if (k0 < keys && pg < pages)
-            for (int i = lane; i < Q4Page<NB>::kHalf / 16; i += 32) cp_async16(half + 16 * i, plane + (size_t)pg * Q4Page<NB>::kBytes + 16 * i);
+            for (int i = part * 32 + lane; i < Q4Page<NB>::kHalf / 16; i += 64) cp_async16(half + 16 * i, plane + (size_t)pg * Q4Page<NB>::kBytes + 16 * i);
         cp_async_commit();
     };
     int phase = 0;
-    fetch((int)blockIdx.x * kPT);
+    if (rows > 0) fetch((int)blockIdx.x * kPT);
     for (int k0 = (int)blockIdx.x * kPT; k0 < keys; k0 += (int)gridDim.x * kPT) {
-        const int key = k0 + tid;
+        const int key = k0 + mine;
         const size_t at = ((size_t)b * p.G + g) * p.maxSeq + key;
-        const float old = key < len ? p.acc[at] : 0.0f;
+        const float old = part == 0 && key < len ? p.acc[at] : 0.0f;
         float add = 0.0f;
         if (rows > 0) {
-            cp_async_wait<0>();
-            __syncwarp();
-            if (k0 / kQ4Page + warp < pages) convert_row<NB, kPT>(half, lane, smem + 2 * S::kTile, tid, 0, 4);
-            else zero_row<NB, kPT>(smem + 2 * S::kTile, tid, 0, 4);
-            __syncwarp();
-            fetch(k0 + (int)gridDim.x * kPT);
             for (int r0 = 0; r0 < rows; r0 += kPT) {
-                const int n = min(rows - r0, kPT);
+                const int n = min(rows - r0, kPT), columns = (n + 15) & ~15;
                 if (k0 == (int)blockIdx.x * kPT || rows > kPT) {         // the queries stay for all tiles if one tile holds them
-                    query_rows<NB>(p, warp, 4, lane, smem, smem + S::kTile, s_factor, [&](int i, int& qm, int& qh, int& qp) {
+                    query_rows<NB>(p, warp, kWThreads / 32, lane, smem, smem + S::kTile, s_factor, columns, [&](int i, int& qm, int& qh, int& qp) {
                         const int row = r0 + min(i, n - 1), of = row / p.ratio, token = room - window + of;
                         qm = first + token; qh = g * p.ratio + row - of * p.ratio; qp = pos + token;
                         return i < n;
                     });
                     __syncthreads();
-                    const int t = room - window + (r0 + tid) / p.ratio;
-                    float2 st = make_float2(0.0f, 1.0f);
-                    if (tid < n) st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(first + t) * p.H + g * p.ratio + (r0 + tid) % p.ratio) * 2);
-                    s_row[tid] = make_float4(s_factor[tid], -st.x, 1.0f / st.y, __int_as_float(tid < n ? len + t : -1));
+                    if (part == 0) {
+                        const int t = room - window + (r0 + mine) / p.ratio;
+                        float2 st = make_float2(0.0f, 1.0f);
+                        if (mine < n) st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(first + t) * p.H + g * p.ratio + (r0 + mine) % p.ratio) * 2);
+                        s_row[mine] = make_float4(s_factor[mine], -st.x, 1.0f / st.y, __int_as_float(mine < n ? len + t : -1));
+                    }
+                }
+                if (r0 == 0) {
+                    cp_async_wait<0>();
+                    __syncthreads();
+                    if (k0 / kQ4Page + (warp & 3) < pages) convert_row<NB, kPT>(half, lane, smem + 2 * S::kTile, mine, 2 * part, 2 * part + 2);
+                    else zero_row<NB, kPT>(smem + 2 * S::kTile, mine, 2 * part, 2 * part + 2);
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
                 __syncthreads();
                 tc_fence_after();
-                if (tid == 0) {
+                if (r0 == 0) fetch(k0 + (int)gridDim.x * kPT);           // everybody has read the pages
+                if (warp == 0) {
+                    const uint32_t lead = elect_one(), idesc = (1u << 4) | ((uint32_t)(columns >> 3) << 17) | ((uint32_t)(kPT >> 4) << 24);
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
                         for (int k = 0; k < HD / 16; k++) {
                             const uint32_t o = (uint32_t)((k >> 2) * (kPT * 128) + (k & 3) * 32);
-                            umma_f16(tmem, desc_k(base + 2 * S::kTile + o), desc_k(base + (1 - h) * S::kTile + o), kIdesc, (h | k) != 0);
+                            umma_f16_by(lead, tmem, desc_k(base + 2 * S::kTile + o), desc_k(base + (1 - h) * S::kTile + o), idesc, (h | k) != 0);
                         }
-                    umma_commit(smem_u32(&s_bar));
+                    umma_commit_by(lead, smem_u32(&s_bar));
                 }
                 __syncwarp();
                 const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_bar), phase & 1, &s_abort, p.error, 350));
                 phase++;
                 tc_fence_after();
 #pragma unroll 1
-                for (int k = 0; ok && k < n; k += 32) {
+                for (int k = part * (kPT / 2); ok && k < min(n, (part + 1) * (kPT / 2)); k += 32) {
                     uint32_t v[32];
-                    tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + k, v);
+                    tmem_ld32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + k, v);
 #pragma unroll
                     for (int i = 0; i < 32; i++) {
                         const float4 q = s_row[k + i];
@@ -739,8 +744,10 @@ __global__ void __launch_bounds__(kWThreads) k_q4_window(const PrefillParams p) 
                 tc_fence_before();
                 __syncthreads();                  // the queries and the sums are read out
             }
+            if (part == 1) s_half[mine] = add;
+            __syncthreads();
         }
-        if (key < keys) p.accOut[at] = old + add;
+        if (part == 0 && key < keys) p.accOut[at] = rows > 0 ? old + (add + s_half[mine]) : old;
     }
     cp_async_wait<0>();
     tc_fence_before();
