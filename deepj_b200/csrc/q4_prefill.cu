@@ -152,52 +152,65 @@ __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, i
         if ((c & 3) >= t0 && (c & 3) < t1) *reinterpret_cast<uint4*>(tile + (c >> 3) * (ROWS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
 }
 
-// Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 8·NB lanes of four values each; `place(row, m, head, position)` says
-// which one row `row` of the first `rows` is, and whether it is one (false: zeros, but the place can be read).  factors[row] makes a sum of products a score in log2 units
-// (NaN where the row holds an infinity or a NaN).  Four rows' loads go out together: one after another they took 20000 cycles a tile.
+// Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 4·NB lanes of eight values each, one 16-byte piece;
+// `place(row, m, head, position)` says which one row `row` of the first `rows` is, and whether it is one (false: zeros, but the place can be read).
+// factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).  Bound by instructions: four values to a lane
+// took 12000 cycles a tile of four heads a token, eight 9000; two rows' loads go out together (one after another 20000).
 template <int NB, typename Place>
 __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, int rows, Place place) {
-    constexpr int HD = 32 * NB, LPR = 8 * NB, RPW = 32 / LPR, AHEAD = 4;
-    const int e = lane % LPR;
-    // this lane's dims 4e … 4e + 3 in the tiles' order: (0, 2) and (1, 3), eight bytes apart
-    const int piece = (e >> 3) * 4 + (e & 3), at = (piece >> 3) * (kPT * 128) + (e & 4);
+    constexpr int HD = 32 * NB, LPR = 4 * NB, RPW = 32 / LPR, AHEAD = 2;
+    const int c = lane % LPR, dim = (c >> 2) * 32 + (c & 3) * 4;         // this lane's piece, word (c % 4, c / 4): its dims dim … dim + 3, and 16 on
+    const float* const q0 = p.qkv + p.q_off + dim;
+    const int at = (c >> 3) * (kPT * 128);
 #pragma unroll 1
     for (int r0 = warp * RPW + lane / LPR; r0 < rows; r0 += AHEAD * warps * RPW) {
-        float4 x[AHEAD];
-        float2 cs[AHEAD], sn[AHEAD];
+        float4 x[AHEAD][2];
+        float2 cs[AHEAD][2], sn[AHEAD][2];
         bool on[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             int m, head, position;
             on[k] = place(min(r0 + k * warps * RPW, rows - 1), m, head, position);
-            const size_t tab = (size_t)position * (HD / 2) + 2 * e;
-            x[k] = *reinterpret_cast<const float4*>(p.qkv + (size_t)m * p.ld + p.q_off + head * HD + 4 * e);
-            cs[k] = *reinterpret_cast<const float2*>(p.cosT + tab);
-            sn[k] = *reinterpret_cast<const float2*>(p.sinT + tab);
+            const float* const from = q0 + (size_t)m * p.ld + head * HD;
+            const size_t tab = (size_t)position * (HD / 2) + (dim >> 1);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                x[k][h] = *reinterpret_cast<const float4*>(from + 16 * h);
+                cs[k][h] = *reinterpret_cast<const float2*>(p.cosT + tab + 8 * h);
+                sn[k][h] = *reinterpret_cast<const float2*>(p.sinT + tab + 8 * h);
+            }
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; k++) {
             const int r = r0 + k * warps * RPW;
-            float4 y = q4_rotate(x[k], cs[k], sn[k]);
-            if (!on[k]) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float most = fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)));
-            if ((y.x + y.y + y.z + y.w) * 0.0f != 0.0f) most = INFINITY;
+            float4 y[2];
+            float most = 0.0f, all = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                y[h] = q4_rotate(x[k][h], cs[k][h], sn[k][h]);
+                most = fmaxf(most, q4_most(y[h]));
+                all += (y[h].x + y[h].y) + (y[h].z + y[h].w);
+            }
+            if (all * 0.0f != 0.0f) most = INFINITY;
 #pragma unroll
             for (int o = 1; o < LPR; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             // the largest value comes to 256 … 512
             most = fmaxf(most, 7.8886091e-31f);
             const int bits = __float_as_int(most) & 0x7f800000;
             const bool fine = most < 1e30f;
-            const float mul = fine ? __int_as_float(0x7f000000 - bits) * 256.0f : 0.0f;
-            if (!fine) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            uint2 h, l;
-            split_half(y.x * mul, y.z * mul, h.x, l.x);
-            split_half(y.y * mul, y.w * mul, h.y, l.y);
+            const float mul = __int_as_float(0x7f000000 - bits) * 256.0f;
+            uint4 h = make_uint4(0, 0, 0, 0), l = h;
+            if (fine && on[k]) {
+                split_half(y[0].x * mul, y[0].z * mul, h.x, l.x);
+                split_half(y[1].x * mul, y[1].z * mul, h.y, l.y);
+                split_half(y[0].y * mul, y[0].w * mul, h.z, l.z);
+                split_half(y[1].y * mul, y[1].w * mul, h.w, l.w);
+            }
             if (r < rows) {
-                const int to = at + r * 128 + (((piece & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint32_t*>(hi + to) = h.x; *reinterpret_cast<uint32_t*>(hi + to + 8) = h.y;
-                *reinterpret_cast<uint32_t*>(lo + to) = l.x; *reinterpret_cast<uint32_t*>(lo + to + 8) = l.y;
-                if (e == 0) factors[r] = fine ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
+                const int to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(hi + to) = h;
+                *reinterpret_cast<uint4*>(lo + to) = l;
+                if (c == 0) factors[r] = fine || !on[k] ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
             }
         }
     }
@@ -288,6 +301,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     __shared__ float s_since[kPT];                // what a row's total has to be multiplied by
     __shared__ float2 s_row[kPT];                 // a row's maximum and sum, for the other blocks of the cluster
     __shared__ volatile int s_parts, s_rows;
+    __shared__ int4 s_place[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);
@@ -316,10 +330,15 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     pdl_launch_dependents();
 
     const int work = blockIdx.x / p.splits, rank = blockIdx.x - work * p.splits, g = work % p.G, tokensPerTile = kPT / p.ratio;
-    int b = 0, first = 0, tokens = 0, t0 = 0, len = 0, pos = 0, room = 0;
-    if (tile_of(p, work / p.G, tokensPerTile, lane, b, first, tokens, t0, len, pos)) room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
+    if (warp == 12) {                             // one warp looks for the tile's place
+        int b = 0, first = 0, tokens = 0, t0 = 0, len = 0, pos = 0, room = 0;
+        if (tile_of(p, work / p.G, tokensPerTile, lane, b, first, tokens, t0, len, pos)) room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos);
+        if (lane == 0) { s_place[0] = make_int4(b, first + t0, t0, room); s_place[1] = make_int4(len + t0, pos + t0, 0, 0); }
+    }
+    __syncthreads();
+    const int b = s_place[0].x, firstToken = s_place[0].y, t0 = s_place[0].z, room = s_place[0].w, len0 = s_place[1].x, pos0 = s_place[1].y;      // of the tile's first token
     const int used = max(0, min(tokensPerTile, room - t0));              // tokens of this tile
-    const int keys = used > 0 ? len + t0 + used : 0, allTiles = (keys + kKT - 1) / kKT;
+    const int keys = used > 0 ? len0 + used : 0, allTiles = (keys + kKT - 1) / kKT;
     // this block's share: tiles from skip on, its keys, pages and tiles count from there
     const int parts = p.splits > 1 ? min(p.splits, max(1, allTiles / p.least)) : 1;
     const int skip = rank < parts ? allTiles * rank / parts : 0, tiles = rank < parts ? allTiles * (rank + 1) / parts - skip : 0;
@@ -329,7 +348,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     auto queries = [&]() {                        // twelve warps lay the queries down
         query_rows<NB>(p, warp, 12, lane, smem, smem + S::kQ, s_factor, kPT, [&](int r, int& qm, int& qh, int& qp) {
             const int t = min(r * inverse >> 16, used - 1);
-            qm = first + t0 + t; qh = g * p.ratio + min(r - t * p.ratio, p.ratio - 1); qp = pos + t0 + t;
+            qm = firstToken + t; qh = g * p.ratio + min(r - t * p.ratio, p.ratio - 1); qp = pos0 + t;
             return r < used * p.ratio;
         });
         fence_proxy_async_smem();
@@ -339,8 +358,8 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     if (warp < 4) {
         const int row = tid, token = row * inverse >> 16, head = g * p.ratio + row - token * p.ratio;
         const bool on = token < used;
-        const int m = first + t0 + token;
-        const int last = on ? len + t0 + token - skip * kKT : -1;         // the row's place in the buffers, its newest key
+        const int m = firstToken + token;
+        const int last = on ? len0 + token - skip * kKT : -1;         // the row's place in the buffers, its newest key
         s_out[row] = on ? p.out + (size_t)m * p.ldo + head * HD : nullptr;
         s_stat[row] = on && p.stats != nullptr && t0 + token >= room - p.window ? m * p.H + head : -1;
         s_since[row] = 1.0f;
