@@ -97,38 +97,46 @@ struct LoadParams {
     const unsigned char* cache; int maxSeq, pages;
     const float* at; const float* end; float* k; float* v; int B, G, T;
 };
+// A lane takes a word: four values and the four 16 on.  Bound by the writes (16 × 32 heads × 1024 rows of 128: 100 µs for 613 MB in and out; 104 with a
+// lane to four values).
 template <int NB>
 __global__ void __launch_bounds__(256) k_q4_load(const LoadParams p) {
-    constexpr int LPR = 8 * NB;                          // lanes of a row, four values each
+    constexpr int LPR = 4 * NB, AHEAD = 4;               // lanes of a row; rows whose loads go out together
     pdl_wait();
     pdl_launch_dependents();
     const int e = threadIdx.x % LPR, bg = blockIdx.y, b = bg / p.G;
     const int at = p.at != nullptr ? (int)p.at[b] : 0, end = min(p.maxSeq, p.end != nullptr ? (int)p.end[b] : p.maxSeq);
     if (at < 0) return;
-    const int j = e >> 3, t = e & 3, shift = (e & 4);    // the four values are one nibble of each byte of word (t, j)
+    const int j = e >> 2, t = e & 3;
+    const unsigned char* const plane = p.cache + (size_t)bg * p.pages * Q4Page<NB>::kBytes;
+    const size_t out = (size_t)bg * p.T * (32 * NB) + 32 * j + 4 * t;
     const int rows = min(p.T, end - at), step = gridDim.x * (256 / LPR);
 #pragma unroll 1
-    for (int i0 = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i0 < rows; i0 += 4 * step) {      // four rows at a time
-        uint32_t w[4][2];
-        float scale[4][2];
+    for (int i0 = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i0 < rows; i0 += AHEAD * step) {
+        uint32_t w[AHEAD][2];
+        unsigned short scale[AHEAD][2];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < AHEAD; k++) {
             const int row = at + min(i0 + k * step, rows - 1), r = row % kQ4Page;
-            const unsigned char* page = p.cache + ((size_t)bg * p.pages + row / kQ4Page) * Q4Page<NB>::kBytes;
+            const unsigned char* page = plane + (size_t)(row / kQ4Page) * Q4Page<NB>::kBytes;
 #pragma unroll
             for (int value = 0; value < 2; value++) {
                 w[k][value] = *reinterpret_cast<const uint32_t*>(page + (value ? Q4Page<NB>::kV : 0) + Q4Page<NB>::word(r, t, j));
-                scale[k][value] = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (r * NB + j) * 2));
+                scale[k][value] = *reinterpret_cast<const unsigned short*>(page + (value ? Q4Page<NB>::kVs : Q4Page<NB>::kKs) + (r * NB + j) * 2);
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < AHEAD; k++)
             if (i0 + k * step < rows) {
-                const size_t to = ((size_t)bg * p.T + i0 + k * step) * (32 * NB) + 4 * e;
+                const size_t to = out + (size_t)(i0 + k * step) * (32 * NB);
 #pragma unroll
                 for (int value = 0; value < 2; value++) {
-                    auto val = [&](int n) { return (float)q4_code(w[k][value], 8 * n + shift) * scale[k][value]; };
-                    __stcs(reinterpret_cast<float4*>((value ? p.v : p.k) + to), make_float4(val(0), val(1), val(2), val(3)));
+                    const float s = __uint_as_float((uint32_t)scale[k][value] << 16);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        auto val = [&](int n) { return (float)q4_code(w[k][value], 8 * n + 4 * h) * s; };
+                        __stcs(reinterpret_cast<float4*>((value ? p.v : p.k) + to + 16 * h), make_float4(val(0), val(1), val(2), val(3)));
+                    }
                 }
             }
     }
@@ -147,9 +155,8 @@ struct EvictParams {
 
 // larger weights → larger numbers; -0 counts as 0, NaN as the least
 __device__ __forceinline__ uint32_t weight_key(float w) {
-    if (w != w) return 0;
     const uint32_t u = __float_as_uint(w + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    return w != w ? 0u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 
 constexpr int kEvictThreads = 512, kEvictBins = 2048;
@@ -216,27 +223,35 @@ __global__ void __launch_bounds__(kEvictThreads) k_q4_select(const EvictParams p
     const bool every = top == old;
     int at = 0, ties = 0;                                // rows placed, rows of the threshold's key met
 #pragma unroll 1
-    for (int i0 = 0; i0 < n; i0 += kEvictThreads) {
-        const int i = i0 + tid;
-        float w = 0.0f;
-        bool over = false, tie = false;
-        if (i < n) {
-            w = acc[i];
-            const uint32_t key = weight_key(w);
-            over = i >= old || every || (top > 0 && key > prefix);
-            tie = !over && top > 0 && key == prefix;
+    for (int i0 = 4 * tid; i0 - 4 * tid < n; i0 += 4 * kEvictThreads) {  // four rows to a thread
+        float w[4];
+        int mine = 0;                                    // rows that stay in the low half, ties in the high half (runs have 2048)
+        unsigned over = 0, tie = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = i0 + k < n ? acc[i0 + k] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + k;
+            const uint32_t key = weight_key(w[k]);
+            const bool stays = i < n && (i >= old || every || (top > 0 && key > prefix)), ties_ = i < n && !stays && top > 0 && key == prefix;
+            over |= (unsigned)stays << k; tie |= (unsigned)ties_ << k;
+            mine += (stays ? 1 : 0) + (ties_ ? 1 << 16 : 0);
         }
-        // one scan for both: rows that stay in the low half, ties in the high half (runs have 512)
         int both;
-        const int sums = before((over ? 1 : 0) + (tie ? 1 << 16 : 0), both);
-        const int tieRank = ties + (sums >> 16), taken = min(max(need - ties, 0), sums >> 16);      // of the ties before this row, those that stay
-        const int place = at + (sums & 0xffff) + taken;
-        if (over || (tie && tieRank < need)) {
-            list[place] = i;
-            p.accOut[bg * p.dstMax + place] = w;         // never behind row i: the rows of this run have been read
-            if (p.kept != nullptr) p.kept[bg * p.budget + place] = (float)i;
+        const int sums = before(mine, both), room = max(need - ties, 0);                        // room: ties of this run that stay
+        int overs = sums & 0xffff, met = sums >> 16;     // of this run before this row
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const bool stays = over >> k & 1, ties_ = tie >> k & 1;
+            if (stays || (ties_ && met < room)) {
+                const int place = at + overs + min(room, met);
+                list[place] = i0 + k;
+                p.accOut[bg * p.dstMax + place] = w[k];  // never behind this row: the rows of this run have been read
+                if (p.kept != nullptr) p.kept[bg * p.budget + place] = (float)(i0 + k);
+            }
+            overs += stays; met += ties_;
         }
-        at += (both & 0xffff) + min(max(need - ties, 0), both >> 16);
+        at += (both & 0xffff) + min(room, both >> 16);
         ties += both >> 16;
     }
     if (g == 0 && tid == 0) p.lenOut[b] = (float)stay;
@@ -287,7 +302,7 @@ __global__ void __launch_bounds__(256) k_q4_move(const MoveParams p) {
 
 template <int NB> void append(const AppendParams& p, cudaStream_t s) { launch_k(k_q4_append<NB>, dim3((unsigned)(((long long)p.M * p.share + 7) / 8)), dim3(256), 0, s, true, p); }
 template <int NB> void load(const LoadParams& p, cudaStream_t s) {
-    const int per = 256 / (8 * NB), blocks = std::min((p.T + per - 1) / per, std::max(1, 16 * g_num_sms / (p.B * p.G)));
+    const int per = 256 / (4 * NB), blocks = std::min((p.T + per - 1) / per, std::max(1, 16 * g_num_sms / (p.B * p.G)));
     launch_k(k_q4_load<NB>, dim3(blocks, p.B * p.G), dim3(256), 0, s, true, p);
 }
 template <int NB> void move(const MoveParams& p, int B, cudaStream_t s) {
