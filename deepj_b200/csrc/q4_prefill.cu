@@ -14,6 +14,8 @@
 // share an SM (half of its tensor and shared memory each: two S/P buffers of 64 columns, O, one tile of keys and one of values).  One block per SM with
 // tiles of 128 keys and two of each took 3900 cycles for 128 keys, where the MMAs take 2048.
 // Where tiles of queries are few, up to four blocks (a cluster) share the keys of one and join their outputs through shared memory, a part of the rows each.
+// Measured: 2048 tokens of 32 heads of 128 88 µs (780 TFLOP/s counting the halves), 6000 of 32/8 heads 510 µs (1150); bound by the chain of a tile (2900 cycles with two
+// blocks on an SM) and by what a block does before its first and after its last tile (25000 cycles).
 // Every wait is bounded (codes 341-350 in the device error word).
 #include <algorithm>
 #include <cmath>

@@ -85,7 +85,8 @@ int deepj_cuda_trace_read(uint64_t* out, int32_t max_launches, int32_t* n_launch
  * captured, [3]=kernel nodes in the last replayed graph, [4]=workspace bytes,
  * [5]=device-side error flag of bounded waits (0 = none; 100 + rank: a tensor-parallel peer's data
  * never arrived; 201-207: a barrier of the tensor-core GEMM; 300-312: the whole-token kernel's grid barrier
- * or rings; 330 - 333: a bulk-copy item of the Q8 GEMV, the several-row kernel, decode attention or the bf16 GEMV never arrived),
+ * or rings; 330 - 333: a bulk-copy item of the Q8 GEMV, the several-row kernel, decode attention or the bf16 GEMV never arrived, 334: a page
+ * of the 4-bit cache; 341 - 350: a barrier of prompt attention over that cache),
  * [6], [7]=bytes and number of released float buffers' blocks that are kept for later buffers (at most 256 MiB and 4096;
  * given back when an allocation of this library fails and by deepj_cuda_shutdown). */
 int deepj_cuda_stats(int64_t* counters, int32_t n);
@@ -314,7 +315,7 @@ int deepj_cuda_latent_alloc(int32_t id, int32_t batch, int32_t max_seq, int32_t 
  *
  *  87 ATTN_DECODE_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, acc, acc_out]
  *                        one token of every sequence: q and k rotated at pos[b] (tables [max_pos][hd/2]), k and v appended as row len[b], softmax
- *                        attention over rows 0..len[b].  acc, acc_out [B][G][max_seq] (or both -1; may be one buffer): acc_out of row j =
+ *                        attention over rows 0..len[b]; out is another buffer than qkv.  acc, acc_out [B][G][max_seq] (or both -1; may be one buffer): acc_out of row j =
  *                        (j < len[b] ? acc : 0) + the softmax weights that the G's query heads give row j; entries beyond len[b] stay
  *  88 ATTN_PACKED_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, starts, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, M, acc, acc_out, window]
  *                        prompts of different lengths: rows starts[b] .. starts[b+1]-1 of the M rows are the tokens of sequence b (none is fine; rows
