@@ -1407,6 +1407,8 @@ int deepj_cuda_kv_alloc_q4(int32_t id, int32_t layers, int32_t batch, int32_t kv
     if (layers <= 0 || batch <= 0 || kv_heads <= 0 || max_seq <= 0) throw std::runtime_error("kv_alloc_q4: dimensions must be positive");
     if (head_dim != 32 && head_dim != 64 && head_dim != 128) throw std::runtime_error("kv_alloc_q4: the head dim must be 32, 64 or 128");
     if (max_seq > 1 << 24) throw std::runtime_error("kv_alloc_q4: lengths travel as floats, which count to 2^24");
+    if (batch > 65535 || (long long)kv_heads * head_dim > 1 << 20) throw std::runtime_error("kv_alloc_q4: too many heads or sequences");      // the ops' limits
+    if ((double)layers * (double)q4_plane_bytes(batch, kv_heads, max_seq, head_dim) > 1e15) throw std::runtime_error("kv_alloc_q4: the cache is larger than any memory");
     if (R.pool.count(id)) throw std::runtime_error("kv_alloc_q4: id " + std::to_string(id) + " already exists");
     Buf b; b.kind = kQ4; b.layers = layers; b.B = batch; b.H = kv_heads; b.maxSeq = max_seq; b.hd = head_dim;
     b.bytes = (size_t)layers * q4_plane_bytes(batch, kv_heads, max_seq, head_dim);

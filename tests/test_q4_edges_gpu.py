@@ -230,3 +230,25 @@ def test_eviction_of_many_sequences(dev, place):  # noqa: F811
             stay = ref.evict(w[b, g], rows_of, budget, recent)
             assert np.array_equal(gk[b, g, :len(stay)], sk[b, g, stay]) and np.array_equal(gv[b, g, :len(stay)], sv[b, g, stay])
             assert np.array_equal(got[b, g, :len(stay)], w[b, g, stay])
+
+
+@pytest.mark.parametrize("layers,B,G,S,hd,message", [
+    (1, 65536, 1, 32, 32, "too many"),
+    (1, 1, 32769, 32, 32, "too many"),
+    (1, 1, 1 << 30, 32, 128, "too many"),
+    (1 << 30, 65535, 8192, 1 << 24, 128, "larger than any memory"),
+    ((1 << 31) - 1, 1, 1, (1 << 24) - 1, 32, "larger than any memory"),
+])
+def test_sizes_that_no_cache_has_are_refused(dev, layers, B, G, S, hd, message):  # noqa: F811
+    with pytest.raises(RuntimeError, match=message):
+        dev.cache(layers, B, G, S, hd)
+
+
+@pytest.mark.parametrize("op", [cg.OP_ATTN_DECODE_Q4, cg.OP_ATTN_PACKED_Q4])
+def test_an_output_among_the_rows_is_refused(dev, op):  # noqa: F811
+    kv = dev.cache(1, 1, 1, 32, 32)
+    x, one, t = dev.buf(np.zeros(4 * 96)), dev.buf(np.zeros(2)), dev.buf(np.zeros(32 * 16))
+    head = [x, 0, 32, 64, 96, kv, 0] + ([one] if op == cg.OP_ATTN_PACKED_Q4 else [])
+    tail = [one, one, t, t, 32, x, 0, 32, 1, 1] + ([1, -1, -1, 0] if op == cg.OP_ATTN_PACKED_Q4 else [-1, -1])
+    with pytest.raises(RuntimeError, match="another buffer"):
+        dev.flush(op, *head, *tail)
