@@ -88,7 +88,9 @@ template <int NB, int HPB> struct DecodeShape {
     static constexpr int kQuery = HPB * 3 * HD;                          // … the queries' digits
     static constexpr int kWarp = kRing + kDigits + kQuery;
     static constexpr size_t kSmem = kDecWarps * kWarp + 64;              // 64: zeros for the columns without a head
-    static constexpr int kResident = HPB == 4 ? 3 : 4;                   // blocks of an SM
+    // blocks of an SM: the stream's registers want room (16 sequences of 32 heads of 128: 37 µs with four, 41 with five); blocks that are many and short want
+    // places (64 sequences of 12 heads of 64: 14.5 with four, 12.5 with five), unless that spills (32 of 16 heads of 128: 10.3 and 12.3)
+    static constexpr int kResident = HPB == 4 ? 3 : 4, kShort = HPB == 1 && NB < 4 ? 5 : kResident;
 };
 
 // What a warp knows of the pages it is at, and its part of a sequence and head.
@@ -322,7 +324,7 @@ __device__ __forceinline__ float weight_of(float mine, float top) { return mine 
 // ───────────── few heads: clusters ─────────────
 // grid (splits, heads of the cache × blocks of query heads, sequences); warps take a split's pages in turn.
 template <int NB, int HPB, bool CLUSTER>
-__global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kResident) k_q4_decode(const DecodeParams p) {
+__global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kShort) k_q4_decode(const DecodeParams p) {
     using S = DecodeShape<NB, HPB>;
     using Page = Q4Page<NB>;
     constexpr int HD = S::HD, kOut = HPB * HD, W = kDecWarps;
