@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
 #pragma unroll
                 for (int i = 0; i < NB; i++)
                     scale[i] = __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(raw_at + 16 * Q4Page<NB>::kRow + ((lane & 15) * NB + i) * 2) << 16);
+                fence_proxy_async_smem();         // the rows are read before the next copy comes over them
                 __syncwarp();
                 request(asked = j + 1);           // everything of this tile is in registers
             }

@@ -252,3 +252,15 @@ def test_an_output_among_the_rows_is_refused(dev, op):  # noqa: F811
     tail = [one, one, t, t, 32, x, 0, 32, 1, 1] + ([1, -1, -1, 0] if op == cg.OP_ATTN_PACKED_Q4 else [-1, -1])
     with pytest.raises(RuntimeError, match="another buffer"):
         dev.flush(op, *head, *tail)
+
+
+@pytest.mark.parametrize("packed,hd,G,R,S,lens,new", [(True, 64, 2, 8, 700, [650, 0], [50, 300]), (True, 128, 8, 4, 400, [0, 100, 0], [300, 260, 129]),
+                                                      (True, 32, 3, 2, 900, [800], [60]), (False, 64, 6, 4, 900, [800, 3, 400], [1, 1, 1])])
+def test_every_repeat_gives_the_same_bits(dev, packed, hd, G, R, S, lens, new):  # noqa: F811
+    """Rows that are read while the copy of the next ones comes over them would show as an output that changes."""
+    rng = np.random.default_rng(11)
+    a = Attention(dev, *drawn(rng, len(lens), G, R, S, hd, sum(new)), lens, new, packed, R)
+    a.check()
+    first = a.run()
+    for _ in range(40):
+        assert np.array_equal(a.run(), first)
