@@ -195,7 +195,6 @@ struct DecodeWarp {
             q4_put_row<NB>(cached, r, false, e, kx, lane < LPR);
             q4_put_row<NB>(cached, r, true, e, vx, lane < LPR);
         }
-        fence_proxy_async_smem();                 // a copy will come over the page
         __syncwarp();
     }
 
@@ -294,6 +293,7 @@ struct DecodeWarp {
                 }
             }
         }
+        fence_proxy_async_smem();                 // the next copy comes over the page
         __syncwarp();                             // the page and the digits are read out
     }
 
