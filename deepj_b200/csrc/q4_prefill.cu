@@ -157,64 +157,54 @@ __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, i
 // Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 4·NB lanes of eight values each, one 16-byte piece;
 // `place(row, m, head, position)` says which one row `row` of the first `rows` is, and whether it is one (false: zeros, but the place can be read).
 // factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).  Bound by instructions: four values to a lane
-// took 12000 cycles a tile of four heads a token, eight 9000; two rows' loads go out together (one after another 20000).
+// took 12000 cycles a tile of four heads a token, eight 9000.  Loads of several rows ahead cost more in code than they give: the roles of a block share
+// the instruction cache (eight prompts of 1500: 303 µs as it is, 307 and 319 with two and three rows ahead).
 template <int NB, typename Place>
 __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, int rows, Place place) {
-    constexpr int HD = 32 * NB, LPR = 4 * NB, RPW = 32 / LPR, AHEAD = 2;
+    constexpr int HD = 32 * NB, LPR = 4 * NB, RPW = 32 / LPR;
     const int c = lane % LPR, dim = (c >> 2) * 32 + (c & 3) * 4;         // this lane's piece, word (c % 4, c / 4): its dims dim … dim + 3, and 16 on
     const float* const q0 = p.qkv + p.q_off + dim;
     const int at = (c >> 3) * (kPT * 128);
 #pragma unroll 1
-    for (int r0 = warp * RPW + lane / LPR; r0 < rows; r0 += AHEAD * warps * RPW) {
-        float4 x[AHEAD][2];
-        float2 cs[AHEAD][2], sn[AHEAD][2];
-        bool on[AHEAD];
+    for (int r = warp * RPW + lane / LPR; r < rows; r += warps * RPW) {
+        int m, head, position;
+        const bool on = place(r, m, head, position);
+        const float* const from = q0 + (size_t)m * p.ld + head * HD;
+        const size_t tab = (size_t)position * (HD / 2) + (dim >> 1);
+        float4 y[2];
+        float2 cs[2], sn[2];
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) {
-            int m, head, position;
-            on[k] = place(min(r0 + k * warps * RPW, rows - 1), m, head, position);
-            const float* const from = q0 + (size_t)m * p.ld + head * HD;
-            const size_t tab = (size_t)position * (HD / 2) + (dim >> 1);
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                x[k][h] = *reinterpret_cast<const float4*>(from + 16 * h);
-                cs[k][h] = *reinterpret_cast<const float2*>(p.cosT + tab + 8 * h);
-                sn[k][h] = *reinterpret_cast<const float2*>(p.sinT + tab + 8 * h);
-            }
+        for (int h = 0; h < 2; h++) {
+            y[h] = *reinterpret_cast<const float4*>(from + 16 * h);
+            cs[h] = *reinterpret_cast<const float2*>(p.cosT + tab + 8 * h);
+            sn[h] = *reinterpret_cast<const float2*>(p.sinT + tab + 8 * h);
         }
+        float most = 0.0f, all = 0.0f;
 #pragma unroll
-        for (int k = 0; k < AHEAD; k++) {
-            const int r = r0 + k * warps * RPW;
-            float4 y[2];
-            float most = 0.0f, all = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                y[h] = q4_rotate(x[k][h], cs[k][h], sn[k][h]);
-                most = fmaxf(most, q4_most(y[h]));
-                all += (y[h].x + y[h].y) + (y[h].z + y[h].w);
-            }
-            if (all * 0.0f != 0.0f) most = INFINITY;
-#pragma unroll
-            for (int o = 1; o < LPR; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // the largest value comes to 256 … 512
-            most = fmaxf(most, 7.8886091e-31f);
-            const int bits = __float_as_int(most) & 0x7f800000;
-            const bool fine = most < 1e30f;
-            const float mul = __int_as_float(0x7f000000 - bits) * 256.0f;
-            uint4 h = make_uint4(0, 0, 0, 0), l = h;
-            if (fine && on[k]) {
-                split_half(y[0].x * mul, y[0].z * mul, h.x, l.x);
-                split_half(y[1].x * mul, y[1].z * mul, h.y, l.y);
-                split_half(y[0].y * mul, y[0].w * mul, h.z, l.z);
-                split_half(y[1].y * mul, y[1].w * mul, h.w, l.w);
-            }
-            if (r < rows) {
-                const int to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4*>(hi + to) = h;
-                *reinterpret_cast<uint4*>(lo + to) = l;
-                if (c == 0) factors[r] = fine || !on[k] ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
-            }
+        for (int h = 0; h < 2; h++) {
+            y[h] = q4_rotate(y[h], cs[h], sn[h]);
+            most = fmaxf(most, q4_most(y[h]));
+            all += (y[h].x + y[h].y) + (y[h].z + y[h].w);
         }
+        if (all * 0.0f != 0.0f) most = INFINITY;
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // the largest value comes to 256 … 512
+        most = fmaxf(most, 7.8886091e-31f);
+        const int bits = __float_as_int(most) & 0x7f800000;
+        const bool fine = most < 1e30f;
+        const float mul = __int_as_float(0x7f000000 - bits) * 256.0f;
+        uint4 h = make_uint4(0, 0, 0, 0), l = h;
+        if (fine && on) {
+            split_half(y[0].x * mul, y[0].z * mul, h.x, l.x);
+            split_half(y[1].x * mul, y[1].z * mul, h.y, l.y);
+            split_half(y[0].y * mul, y[0].w * mul, h.z, l.z);
+            split_half(y[1].y * mul, y[1].w * mul, h.w, l.w);
+        }
+        const int to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(hi + to) = h;
+        *reinterpret_cast<uint4*>(lo + to) = l;
+        if (c == 0) factors[r] = fine || !on ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
     }
 }
 
