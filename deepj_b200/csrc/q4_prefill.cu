@@ -175,8 +175,8 @@ __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int
         float2 cs[2], sn[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            y[h] = *reinterpret_cast<const float4*>(from + 16 * h);
-            cs[h] = *reinterpret_cast<const float2*>(p.cosT + tab + 8 * h);
+            y[h] = __ldcg(reinterpret_cast<const float4*>(from + 16 * h));
+            cs[h] = *reinterpret_cast<const float2*>(p.cosT + tab + 8 * h);      // the heads of a token share them: through L1
             sn[h] = *reinterpret_cast<const float2*>(p.sinT + tab + 8 * h);
         }
         float most = 0.0f, all = 0.0f;
@@ -252,9 +252,9 @@ __device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int to
     for (int b0 = 0; b0 < p.B; b0 += 32) {
         int from = 0, n = 0, l = 0, q = 0;
         if (b0 + lane < p.B) {
-            from = max(0, (int)p.starts[b0 + lane]);
-            n = max(0, min(p.M, (int)p.starts[b0 + lane + 1]) - from);
-            l = (int)p.len[b0 + lane]; q = (int)p.pos[b0 + lane];
+            from = max(0, (int)__ldcg(p.starts + b0 + lane));
+            n = max(0, min(p.M, (int)__ldcg(p.starts + b0 + lane + 1)) - from);
+            l = (int)__ldcg(p.len + b0 + lane); q = (int)__ldcg(p.pos + b0 + lane);
         }
         const int tiles = (n + tokensPerTile - 1) / tokensPerTile;
         int upto = tiles;
@@ -318,9 +318,8 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    pdl_wait();
-    pdl_launch_dependents();
 
+    // The kernel before is the append, which has passed its own wait: all but the rows that it writes is complete, so the queries are laid down before it ends.
     const int work = blockIdx.x / p.splits, rank = blockIdx.x - work * p.splits, g = work % p.G, tokensPerTile = kPT / p.ratio;
     if (warp == 12) {                             // one warp looks for the tile's place
         int b = 0, first = 0, tokens = 0, t0 = 0, len = 0, pos = 0, room = 0;
@@ -346,6 +345,16 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(qReady);
+    };
+    const unsigned char* const plane = p.cache + (((size_t)b * p.G + g) * p.pages + 2 * skip) * Q4Page<NB>::kBytes;
+    auto request = [&](int c, int j) {            // rows of tile j for conversion warp c: its sixteen of keys (c < 4) or values
+        const int w = c & 3;
+        if (j >= tiles || 2 * j + (w >> 1) >= pages) return;
+        const unsigned char* const half = plane + (size_t)(2 * j + (w >> 1)) * Q4Page<NB>::kBytes + (c >= 4 ? Q4Page<NB>::kV : 0);
+        const uint32_t to = smem_u32(smem + S::kRawAt + c * S::kRaw);
+        mbar_arrive_expect_tx(bar(c), S::kRaw);
+        bulk_g2s(to, half + (w & 1) * (16 * Q4Page<NB>::kRow), 16 * Q4Page<NB>::kRow, bar(c));
+        bulk_g2s(to + 16 * Q4Page<NB>::kRow, half + Q4Page<NB>::kKs + (w & 1) * (32 * NB), 32 * NB, bar(c));
     };
     if (warp < 4) {
         const int row = tid, token = row * inverse >> 16, head = g * p.ratio + row - token * p.ratio;
@@ -514,19 +523,10 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     } else if (warp < 12) {
         const bool value = warp >= 8;
         const int w = warp & 3, row = 16 * w + (lane & 15), t0w = lane >> 4 << 1;        // row of the tile, first of this lane's two pieces
-        unsigned char* const raw_at = smem + S::kRawAt + (warp - 4) * S::kRaw;
+        const unsigned char* const raw_at = smem + S::kRawAt + (warp - 4) * S::kRaw;
         unsigned char* const tile = smem + (value ? S::kVAt : S::kKAt);
         const uint32_t arrived = bar(warp - 4);
-        const unsigned char* from = p.cache + (((size_t)b * p.G + g) * p.pages + 2 * skip + (w >> 1)) * Q4Page<NB>::kBytes + (value ? Q4Page<NB>::kV : 0);
-        auto request = [&](int j) {               // this warp's rows of tile j
-            if (lane == 0 && j < tiles && 2 * j + (w >> 1) < pages) {
-                const unsigned char* const page = from + (size_t)(2 * j) * Q4Page<NB>::kBytes;
-                mbar_arrive_expect_tx(arrived, S::kRaw);
-                bulk_g2s(smem_u32(raw_at), page + (w & 1) * (16 * Q4Page<NB>::kRow), 16 * Q4Page<NB>::kRow, arrived);
-                bulk_g2s(smem_u32(raw_at) + 16 * Q4Page<NB>::kRow, page + Q4Page<NB>::kKs + (w & 1) * (32 * NB), 32 * NB, arrived);
-            }
-        };
-        request(0);
+        const unsigned char* const from = plane + (size_t)(w >> 1) * Q4Page<NB>::kBytes + (value ? Q4Page<NB>::kV : 0) + (w & 1) * (16 * Q4Page<NB>::kRow);
         if (tiles > 0) queries();
         int j = 0, asked = 0;                     // asked: the last tile whose rows were
 #pragma unroll 1
@@ -543,7 +543,12 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                     scale[i] = __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(raw_at + 16 * Q4Page<NB>::kRow + ((lane & 15) * NB + i) * 2) << 16);
                 fence_proxy_async_smem();         // the rows are read before the next copy comes over them
                 __syncwarp();
-                request(asked = j + 1);           // everything of this tile is in registers
+                asked = j + 1;                    // everything of this tile is in registers
+                if (lane == 0 && j + 1 < tiles && 2 * (j + 1) + (w >> 1) < pages) {
+                    mbar_arrive_expect_tx(arrived, S::kRaw);
+                    bulk_g2s(smem_u32(raw_at), from + (size_t)(j + 1) * (2 * Q4Page<NB>::kBytes), 16 * Q4Page<NB>::kRow, arrived);
+                    bulk_g2s(smem_u32(raw_at) + 16 * Q4Page<NB>::kRow, from + (size_t)(j + 1) * (2 * Q4Page<NB>::kBytes) + Q4Page<NB>::kKs - (w & 1) * (16 * Q4Page<NB>::kRow - 32 * NB), 32 * NB, arrived);
+                }
             }
             if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait_long(value ? vEmpty : kEmpty, (j - 1) & 1, &s_abort, p.error, 344))) break;
             if (there) convert_pieces<NB, kKT>(words, scale, tile, row, t0w);
@@ -556,6 +561,10 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     } else {
         // The whole warp walks the loop and one lane's predicate issues: in one lane's branch every operand would be moved into a uniform register first (70
         // cycles an MMA).  Rolled: what is issued has to come from the instruction cache in time.
+        pdl_wait();
+        pdl_launch_dependents();
+        if (lane < 8) request(lane, 0);
+        __syncwarp();
         const uint32_t lead = elect_one();
         auto waited = [&](uint32_t on, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait_long(on, parity, &s_abort, p.error, code)); };
         auto scores = [&](int j) {
@@ -678,9 +687,16 @@ __global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_wait();
-    pdl_launch_dependents();
-    const int first = max(0, (int)p.starts[b]), tokens = max(0, min(p.M, (int)p.starts[b + 1]) - first), len = (int)p.len[b], pos = (int)p.pos[b];
+    // The kernel before has passed its own wait: all but the statistics that it writes is complete.
+    bool waited = false;
+    auto wait = [&]() {
+        if (waited) return;
+        pdl_wait();
+        pdl_launch_dependents();
+        waited = true;
+    };
+    if (p.M == 0) wait();                         // there is no such kernel then
+    const int first = max(0, (int)__ldcg(p.starts + b)), tokens = max(0, min(p.M, (int)__ldcg(p.starts + b + 1)) - first), len = (int)__ldcg(p.len + b), pos = (int)__ldcg(p.pos + b);
     const bool there = len >= 0 && len < p.maxSeq && pos >= 0 && pos < p.maxPos;
     const int room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos), keys = there ? len + room : 0, pages = (keys + kQ4Page - 1) / kQ4Page;
     const int window = min(p.window, room), rows = window * p.ratio;
@@ -698,7 +714,7 @@ __global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams 
     for (int k0 = (int)blockIdx.x * kPT; k0 < keys; k0 += (int)gridDim.x * kPT) {
         const int key = k0 + mine;
         const size_t at = ((size_t)b * p.G + g) * p.maxSeq + key;
-        const float old = part == 0 && key < len ? p.acc[at] : 0.0f;
+        const float old = part == 0 && key < len ? __ldcg(p.acc + at) : 0.0f;
         float add = 0.0f;
         if (rows > 0) {
             for (int r0 = 0; r0 < rows; r0 += kPT) {
@@ -709,11 +725,12 @@ __global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams 
                         qm = first + token; qh = g * p.ratio + row - of * p.ratio; qp = pos + token;
                         return i < n;
                     });
+                    wait();
                     __syncthreads();
                     if (part == 0) {
                         const int t = room - window + (r0 + mine) / p.ratio;
                         float2 st = make_float2(0.0f, 1.0f);
-                        if (mine < n) st = *reinterpret_cast<const float2*>(p.stats + ((size_t)(first + t) * p.H + g * p.ratio + (r0 + mine) % p.ratio) * 2);
+                        if (mine < n) st = __ldcg(reinterpret_cast<const float2*>(p.stats + ((size_t)(first + t) * p.H + g * p.ratio + (r0 + mine) % p.ratio) * 2));
                         s_row[mine] = make_float4(s_factor[mine], -st.x, 1.0f / st.y, __int_as_float(mine < n ? len + t : -1));
                     }
                 }
@@ -759,8 +776,10 @@ __global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams 
             if (part == 1) s_half[mine] = add;
             __syncthreads();
         }
+        wait();
         if (part == 0 && key < keys) p.accOut[at] = rows > 0 ? old + (add + s_half[mine]) : old;
     }
+    wait();
     cp_async_wait<0>();
     tc_fence_before();
     __syncthreads();

@@ -264,3 +264,46 @@ def test_every_repeat_gives_the_same_bits(dev, packed, hd, G, R, S, lens, new): 
     first = a.run()
     for _ in range(40):
         assert np.array_equal(a.run(), first)
+
+
+@pytest.mark.parametrize("packed,G,R,S,lens,new,window", [(True, 2, 1, 300, [0, 40], [33, 130], 8), (True, 8, 4, 600, [0, 100, 7], [200, 260, 129], 0), (True, 1, 2, 3000, [2500, 0], [40, 9], 20),
+                                                          (False, 4, 2, 600, [500, 3, 77], [1, 1, 1], 1)])
+def test_inputs_that_change_right_before_the_op(dev, packed, G, R, S, lens, new, window):  # noqa: F811
+    """Rows, tables, lengths, positions, starts and weights of two problems are copied in turn into one set of buffers by the ops before: a block that starts
+    before the kernel in front of it has ended has to see all of them."""
+    rng = np.random.default_rng(12)
+    hd, H, B, M = 64, G * R, len(lens), sum(new)
+    width, parts = (H + 2 * G) * hd, []
+    for turn in range(2):
+        n = np.asarray(lens, np.float32) if turn == 0 else np.maximum(np.asarray(lens, np.float32) - 3, 0)
+        cos, sin = tables(S + 50, hd)
+        if turn:
+            cos, sin = np.ascontiguousarray(cos[::-1]), np.ascontiguousarray(sin[::-1])
+        order = new if turn == 0 else new[::-1]
+        parts.append([rows(rng, M, width), np.concatenate(([0], np.cumsum(order))).astype(np.float32), n, n + 5 * turn, cos, sin, rng.random((B, G, S)).astype(np.float32)])
+    kv = dev.cache(1, B, G, S, hd)
+    dev.store(kv, 0, rows(rng, B, G, S, hd), rows(rng, B, G, S, hd))
+    shared = [dev.buf(np.zeros(a.size)) for a in parts[0]]
+    held = [[dev.buf(a) for a in p] for p in parts]
+    outs, weights = [dev.buf(np.zeros(M * H * hd)) for _ in parts], [dev.buf(np.zeros(B * G * S)) for _ in parts]
+
+    def words(turn):
+        x, starts, n, pos, cos, sin, acc = shared
+        copies = [w for to, of, a in zip(shared, held[turn], parts[turn]) for w in (cg.OP_COPY, of, 0, to, 0, a.size)]
+        tail = [n, pos, cos, sin, S + 50, outs[turn], 0, H * hd, B, H]
+        seen = [acc, weights[turn]] if window else [-1, -1]
+        where = [x, 0, H * hd, (H + G) * hd, width, kv, 0]
+        return copies + ([cg.OP_ATTN_PACKED_Q4] + where + [starts] + tail + [M] + seen + [window] if packed else [cg.OP_ATTN_DECODE_Q4] + where + tail + seen)
+
+    def results():
+        return [dev.get(i, (M * H * hd,)).tobytes() for i in outs] + [dev.get(i, (B * G * S,)).tobytes() for i in weights]
+
+    for _ in range(2):                                               # the rows that both write are the same again before each of them
+        for turn in range(2):
+            for w in np.split(np.arange(0, 7 * 6), 7):
+                dev.flush(*[words(turn)[i] for i in w])              # a copy to a flush: nothing is close behind anything
+            dev.flush(*words(turn)[42:])
+    alone = results()
+    for _ in range(12):
+        dev.flush(*words(0), *words(1))
+        assert results() == alone
