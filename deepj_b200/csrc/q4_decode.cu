@@ -752,10 +752,10 @@ DecodePlan decode_plan(const Q4AttnArgs& a) {
     d.pages = (a.maxSeq + kQ4Page - 1) / kQ4Page;
     d.blocks = (d.perBlock == 4 ? 3 : 4) * g_num_sms;                    // all that are resident at once
     const long long heads = (long long)a.B * a.G * d.headBlocks;
-    // Clusters of up to eight where they fit onto the chip together.  Pages in a row where a block would have more than 32 of a head (16 sequences of
+    // Clusters of up to eight where they fit onto the chip together, until a warp has a page (16 heads of 10 pages: 5.5 µs with two blocks to a head, 4.8 with four).  Pages in a row where a block would have more than 32 of a head (16 sequences of
     // 32 heads with 65 each 46 µs a block each, 41 in a row; 64 of 12 heads with 7 each 15 and 18.5).
     d.splits = 1;
-    while (d.splits < kDecCluster && d.splits * 2 * kDecWarps <= d.pages + kDecWarps - 1 && heads * d.splits * 2 <= d.blocks) d.splits *= 2;
+    while (d.splits < kDecCluster && d.splits * kDecWarps < d.pages && heads * d.splits * 2 <= d.blocks) d.splits *= 2;
     d.stream = d.pages > 8 * kDecWarps * d.splits || (a.accOut != nullptr && d.headBlocks > 1);
     d.scores = a.accOut != nullptr ? (size_t)a.B * a.H * d.pages * kQ4Page : 0;
     if (d.stream) {
