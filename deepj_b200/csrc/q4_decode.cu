@@ -82,15 +82,15 @@ template <int NB> __device__ __forceinline__ void lds_scales(float (&s)[NB], con
 
 template <int NB, int HPB> struct DecodeShape {
     static constexpr int HD = 32 * NB, NT = (HPB + 1) / 2, CH = HPB == 1 ? 1 : 2;      // tiles of heads, heads of a tile
-    static constexpr int kStages = NB == 4 ? 2 : NB == 2 ? 4 : 6;
+    static constexpr int kStages = NB == 4 ? 2 : NB == 2 ? 3 : 6;
     static constexpr int kRing = kStages * Q4Page<NB>::kBytes;           // of a warp
     static constexpr int kDigits = NB * HPB * 96;                        // … [block][head][digit][32 rows]
     static constexpr int kQuery = HPB * 3 * HD;                          // … the queries' digits
     static constexpr int kWarp = kRing + kDigits + kQuery;
     static constexpr size_t kSmem = kDecWarps * kWarp + 64;              // 64: zeros for the columns without a head
     // blocks of an SM: the stream's registers want room (16 sequences of 32 heads of 128: 37 µs with four, 41 with five); blocks that are many and short want
-    // places (64 sequences of 12 heads of 64: 14.5 with four, 12.5 with five), unless that spills (32 of 16 heads of 128: 10.3 and 12.3)
-    static constexpr int kResident = HPB == 4 ? 3 : 4, kShort = HPB == 1 && NB < 4 ? 5 : kResident;
+    // places (64 sequences of 12 heads of 64: 14.4 with four, 12.3 with five, 10.3 with six), unless that spills (32 of 16 heads of 128: 10.3 and, with five, 12.3)
+    static constexpr int kResident = HPB == 4 ? 3 : 4, kShort = HPB == 1 && NB < 4 ? 6 : kResident;
 };
 
 // What a warp knows of the pages it is at, and its part of a sequence and head.
