@@ -128,7 +128,7 @@ int deepj_cuda_kv_alloc_f16(int32_t kv_id, int32_t layers, int32_t batch, int32_
  * 128.  Every row is cut into blocks of 32 values: scale = bf16(max|w| * fp32(1/7)), at least 2^-17 and at most 2^13 (0 for a block of zeros), code =
  * clamp(round-half-even(w / scale), -7, 7), NaN -> 0; a row reads back as code * scale.  Keys are rotated in fp32 before they are quantized.
  * 1.125 * head_dim bytes hold a key and a value row.  How many rows a sequence has is the caller's (`len`, a float buffer), apart from the
- * position its next token is rotated at (`pos`): after an eviction the two differ.  max_seq <= 2^24. */
+ * position its next token is rotated at (`pos`): after an eviction the two differ.  max_seq <= 2^24, batch <= 65535, kv_heads * head_dim <= 2^20. */
 int deepj_cuda_kv_alloc_q4(int32_t kv_id, int32_t layers, int32_t batch, int32_t kv_heads, int32_t max_seq, int32_t head_dim);
 
 /* Device address and size of a float buffer, for other libraries on the device (no copy).  Work of other streams on it is the caller's to order:
