@@ -46,7 +46,8 @@ struct PrefillParams {
 constexpr int kMaxSplits = 4;
 // Tiles whose values are summed in tensor memory.  Those sums are cut off, not rounded: values of one sign lose 5.6e-9 of their sum a key, 3.4e-5 at 6000 keys.
 // So a sum of 16 tiles goes to memory, where it is added rounded: 6e-6 at any length (32 tiles: 1.1e-5), for 3 % of the time at 1500 keys and 6 % at 6000
-// (emptied every 8 tiles: 12 % and 14 %).
+// (emptied every 8 tiles: 12 % and 14 %).  The sums of the weights go the same way, a tile's and then sixteen tiles' by themselves: a chain of 16 thousand
+// equal weights was off by 2e-4.
 constexpr int kSegment = 16;
 
 constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     __shared__ float* s_out[kPT];                 // a row's place in the output; null: no row of a token
     __shared__ int s_stat[kPT];                   // and in the statistics, or -1
     __shared__ float s_since[kPT];                // what a row's total has to be multiplied by
+    __shared__ float s_weights[kPT];              // a row's total of weights
     __shared__ float2 s_row[kPT];                 // a row's maximum and sum, for the other blocks of the cluster
     __shared__ volatile int s_parts, s_rows;
     __shared__ int4 s_place[2];
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         s_since[row] = 1.0f;
         if (row == 0) { s_parts = parts; s_rows = used * p.ratio; }          // the arrival for the queries publishes them
         float c = 1.0f, top = -INFINITY;
-        float2 sums = make_float2(0.0f, 0.0f);
+        float weights = 0.0f;                     // of the tiles since the last total
         if (tiles > 0) {
             queries();
             mbar_wait_long(qReady, 0, &s_abort, p.error, 349);
@@ -405,6 +407,8 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                         }
                     }
             }
+            s_weights[tid] = fresh ? weights : fmaf(s_weights[tid], since, weights);
+            weights = 0.0f;
             s_since[tid] = 1.0f;
         };
 #pragma unroll 1
@@ -453,12 +457,13 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                         tmem_st32(mine + kO + k, o);
                     }
                 }
-                sums.x *= f; sums.y *= f;
+                weights *= f;
                 s_since[tid] *= f;
                 top = now;
             }
             const float shift = top > -INFINITY ? -top : 0.0f;           // a row without keys yet: every weight is 2^-inf
             const float2 c2 = make_float2(c, c), shift2 = make_float2(shift, shift), minus = make_float2(-1.0f, -1.0f);
+            float2 sums = make_float2(0.0f, 0.0f);
 #pragma unroll 1
             for (int q = 0; q < kKT / 32; q++) {
                 uint32_t v[32], w[32];
@@ -480,6 +485,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pReady(j & 1));
+            weights += sums.x + sums.y;
         }
         if (tiles > 0) {
             // through shared memory (the queries and keys have been read out), so that a warp stores whole rows
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
             const float since = s_since[tid];
             const int there = min(32, s_rows - warp * 32);
             const bool shared = s_parts > 1;
-            const float sum = sums.x + sums.y, inv = shared ? 1.0f : 1.0f / sum;
+            const float sum = tiles > kSegment ? fmaf(s_weights[tid], since, weights) : weights, inv = shared ? 1.0f : 1.0f / sum;
             if (shared) s_row[row] = make_float2(top, sum);
 #pragma unroll 1
             for (int k = 0; ok && k < HD; k += 32) {

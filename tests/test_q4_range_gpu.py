@@ -1,0 +1,70 @@
+"""Attention over the 4-bit cache where the numbers are far apart or add up: sums of thousands of equal weights."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import q4_ref as ref
+from deepj_b200 import _lib
+from deepj_b200 import compute_graph as cg
+from test_q4_cache_gpu import FILL, dev, rows, tables  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(dev):  # noqa: F811
+    yield
+    stats = (ctypes.c_int64 * 8)()
+    _lib.check(dev.rt.lib.deepj_cuda_stats(stats, 8))
+    assert stats[5] == 0
+
+
+def attend(dev, K, V, qkv, n, packed, R=1, window=0):  # noqa: F811
+    """One sequence of n cached rows and M new tokens (a step: one) → outputs [M][H][hd], accumulated weights [G][n + M] or None.  Positions are 0: the tables'
+    first rows do not rotate."""
+    G, _, hd = K.shape
+    M, H, S = qkv.shape[0], K.shape[0] * R, n + qkv.shape[0]
+    kv = dev.cache(1, 1, G, S, hd)
+    dev.store(kv, 0, K[None], V[None])
+    out = dev.buf(np.full(M * H * hd, FILL))
+    a, ao = (dev.buf(np.zeros(G * S)), dev.buf(np.full(G * S, FILL))) if window else (-1, -1)
+    ones, none = dev.buf(np.ones(max(M, 1) * hd // 2)), dev.buf(np.zeros(max(M, 1) * hd // 2))
+    head = [dev.buf(qkv), 0, H * hd, (H + G) * hd, qkv.shape[1], kv, 0]
+    tail = [dev.buf([n]), dev.buf([0]), ones, none, M, out, 0, H * hd, 1, H]
+    if packed:
+        dev.flush(cg.OP_ATTN_PACKED_Q4, *head, dev.buf([0, M]), *tail, M, a, ao, window)
+    else:
+        dev.flush(cg.OP_ATTN_DECODE_Q4, *head, *tail, a, ao)
+    return dev.get(out, (M, H, hd)), dev.get(ao, (G, S)) if window else None
+
+
+def one_above(G, n, hd, M, nats, sink, others):
+    """n cached rows: the first one's score is `nats` above those of all others, which are 0; values `sink` and `others`.  Returns K, V, qkv and the score."""
+    K, V = np.zeros((G, n, hd), np.float32), np.full((G, n, hd), others, np.float32)
+    K[:, 0], V[:, 0] = 7.0, sink                                     # scale 1, code 7: stored as they are
+    qkv = np.zeros((M, 3 * G * hd), np.float32)
+    qkv[:, :G * hd] = nats / (7.0 * np.sqrt(hd))                     # times 7, hd of them, over the root of hd
+    qkv[:, 2 * G * hd:] = others
+    score = float(qkv[0, 0]) * 7.0 * np.sqrt(hd)
+    return K, V, qkv, score
+
+
+def relative(score):
+    """What a weight, a sum of weights and a product with values may be off, relative to themselves.  Operands carry 22 bits: a score is off by 2^-21 of its
+    terms' magnitudes, twice (two weights of a quotient); exponential and quotient 2^-20.  The tensor cores cut an fp32 sum off once for 16 keys and each half of the
+    weights, 128 times 2^-23 until it is added up rounded; the sums of weights are 64 additions of 2^-24 one behind the other at most."""
+    return 2 * 2.0 ** -21 * abs(score) + 2.0 ** -20 + 128 * 2.0 ** -23 + 64 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("G,n", [(2, 16000), (160, 16000)])
+@pytest.mark.parametrize("nats", [0.3, 0.7, 2.9])
+def test_sums_of_equal_weights(dev, packed, G, n, nats):  # noqa: F811
+    """All values are equal, so the output is that value: sums that drift apart show.  The weights of a chain of equal ones are all rounded the same way."""
+    hd, M = 32, 2 if packed else 1
+    K, V, qkv, score = one_above(G, n, hd, M, nats, 7.0, 7.0)
+    got, weights = attend(dev, K, V, qkv, n, packed, window=1)
+    assert np.all(np.abs(got / 7.0 - 1.0) <= relative(score)), float(np.abs(got / 7.0 - 1.0).max() / relative(score))
+    rest = (n + M - 1) * np.exp(-score)
+    assert np.all(np.abs(weights[:, 1:] * (1.0 + rest) * np.exp(score) - 1.0) <= relative(score)), float(np.abs(weights[:, 1:] * (1.0 + rest) * np.exp(score) - 1.0).max())
