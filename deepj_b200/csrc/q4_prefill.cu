@@ -3,10 +3,10 @@
 // A block takes 128 query rows of one key/value head: 128 / R consecutive tokens of one sequence times the R query heads that share the head, so that a
 // key or value is brought and converted once for all of them.  It walks the cached rows in tiles of 64:
 //   S = Q·Kᵀ    Q in fp16 halves hi + lo of the rotated row times a power of two (22 bits); a stored key, code · scale, is exact in fp16: two MMAs
-//   P = 2^(S·c − m) per row, in halves hi + lo again, written over S in tensor memory, from where it is the A operand of
+//   P = 2^(S·c − m + 9) per row, in halves hi + lo again, written over S in tensor memory, from where it is the A operand of
 //   O += P·V    with O in tensor memory as well
 //   warps 0-3   a thread is a row: running maximum and sum of the softmax in fp32, no exchange between lanes.  O is multiplied by the change of the
-//               maximum only when that grew by more than 2^8: until then P is larger than one, which fp16 and the fp32 sums have room for
+//               maximum only when a weight would leave fp16 (see kLift)
 //   warps 4-11  four for keys, four for values, sixteen rows of a tile each: bulk copies into a place of their own, the codes into registers, and when the
 //               tile is free 4-bit codes → fp16 with 128-byte swizzle
 //   warp 12     issues the MMAs: Q·K of the next tile before P·V of this one
@@ -37,7 +37,7 @@ struct PrefillParams {
     const unsigned char* cache; int maxSeq, pages;
     const float* starts; const float* len; const float* pos; const float* cosT; const float* sinT; int maxPos;
     float* out; int ldo; int B, H, G, ratio, M; float scale;            // scale: 1/sqrt(hd) · log2(e)
-    float* stats; int window;                     // [M][H][2] maximum (log2) and sum of the last `window` tokens' rows, or null
+    float* stats; int window;                     // [M][H][2] base (log2) and sum of the weights to it of the last `window` tokens' rows, or null
     const float* acc; float* accOut;
     int* error;
     float* totals;                                // [block][128][hd] for the blocks of clusters
@@ -49,6 +49,10 @@ constexpr int kMaxSplits = 4;
 // (emptied every 8 tiles: 12 % and 14 %).  The sums of the weights go the same way, a tile's and then sixteen tiles' by themselves: a chain of 16 thousand
 // equal weights was off by 2e-4.
 constexpr int kSegment = 16;
+// A row's weights are taken to a base 2^9 below its maximum, P up to 2^9, and the base stays until one would be above 2^15, the last power of two in fp16.  Steps of
+// fp16 end at 2^-24: with the maximum at 2^9, a weight is off by at most 2^-33 of the row's largest (two halves, half a step each).  With the maximum at 1, weights under
+// 2^-14 of it kept 10 bits and fewer, those under 2^-25 none: thousands of keys 10 … 18 nats below one were off by up to all of their sum.
+constexpr float kLift = 9.0f, kTop = 15.0f;
 
 constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
 template <int NB> struct PrefillShape {
@@ -293,7 +297,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
     __shared__ int s_stat[kPT];                   // and in the statistics, or -1
     __shared__ float s_since[kPT];                // what a row's total has to be multiplied by
     __shared__ float s_weights[kPT];              // a row's total of weights
-    __shared__ float2 s_row[kPT];                 // a row's maximum and sum, for the other blocks of the cluster
+    __shared__ float2 s_row[kPT];                 // a row's base and sum, for the other blocks of the cluster
     __shared__ volatile int s_parts, s_rows;
     __shared__ int4 s_place[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
         s_stat[row] = on && p.stats != nullptr && t0 + token >= room - p.window ? m * p.H + head : -1;
         s_since[row] = 1.0f;
         if (row == 0) { s_parts = parts; s_rows = used * p.ratio; }          // the arrival for the queries publishes them
-        float c = 1.0f, top = -INFINITY;
+        float c = 1.0f, top = -INFINITY;          // top: the base
         float weights = 0.0f;                     // of the tiles since the last total
         if (tiles > 0) {
             queries();
@@ -442,9 +446,9 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 most = fmaxf(m2[0], m2[1]);
             }
             most *= c;
-            const bool grown = most > top + 8.0f;                        // also the first keys of a row
+            const bool grown = most > top + kTop;                        // also the first keys of a row
             if (__any_sync(0xffffffffu, grown)) {
-                const float now = grown ? most : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
+                const float now = grown ? most - kLift : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
                 if (j % kSegment > 0) {
                     if (!__all_sync(0xffffffffu, mbar_wait_long(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
                     tc_fence_after();
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams 
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
     __shared__ float s_factor[kPT], s_half[kPT];  // s_half: the sums of the second half of the queries
-    __shared__ float4 s_row[kPT];                 // factor, maximum, 1 / sum, newest key of every query row
+    __shared__ float4 s_row[kPT];                 // factor, -base, 1 / sum, newest key of every query row
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, mine = tid & (kPT - 1), part = tid / kPT, g = blockIdx.y, b = blockIdx.z;
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     unsigned char* const smem = smem_raw + (base - raw);

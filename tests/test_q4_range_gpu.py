@@ -1,4 +1,5 @@
-"""Attention over the 4-bit cache where the numbers are far apart or add up: sums of thousands of equal weights."""
+"""Attention over the 4-bit cache where the numbers are far apart or add up: a key that takes nearly all of the weight above thousands that share the rest,
+sums of thousands of equal weights."""
 import ctypes
 
 import numpy as np
@@ -55,6 +56,25 @@ def relative(score):
     terms' magnitudes, twice (two weights of a quotient); exponential and quotient 2^-20.  The tensor cores cut an fp32 sum off once for 16 keys and each half of the
     weights, 128 times 2^-23 until it is added up rounded; the sums of weights are 64 additions of 2^-24 one behind the other at most."""
     return 2 * 2.0 ** -21 * abs(score) + 2.0 ** -20 + 128 * 2.0 ** -23 + 64 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("G,n", [(2, 4000), (2, 16000), (160, 4000), (160, 16000)])
+@pytest.mark.parametrize("nats", [10.0, 17.4, 18.0])
+def test_many_small_weights_below_a_large_one(dev, packed, G, n, nats):  # noqa: F811
+    """The large weight's value is zero, the others' are equal: the output is what is left of the small weights."""
+    hd, M = 32, 3 if packed else 1
+    K, V, qkv, score = one_above(G, n, hd, M, nats, 0.0, 7.0)
+    got, weights = attend(dev, K, V, qkv, n, packed, window=1)
+    for t in range(M):
+        rest = (n - 1 + t + 1) * np.exp(-score)
+        want = 7.0 * rest / (1.0 + rest)
+        # in prompts a weight is two fp16 halves of 2^9 times it, whose steps end at 2^-24
+        tol = want * relative(score) + 7.0 * (n + t) * 2.0 ** -33
+        assert np.all(np.abs(got[t] - want) <= tol), (t, float(np.abs(got[t] - want).max() / tol), float(got[t].flat[0]), want)
+    rest = (n + M - 1) * np.exp(-score)
+    assert np.all(np.abs(weights[:, 0] * (1.0 + rest) - 1.0) <= relative(score))
+    assert np.all(np.abs(weights[:, 1:] * (1.0 + rest) * np.exp(score) - 1.0) <= relative(score))
 
 
 @pytest.mark.parametrize("packed", [True, False])
