@@ -147,7 +147,7 @@ struct DecodeWarp {
     // A head's query, rotated, in fixed point of its largest value → its digits at `to`; returns the factor of its sums, in log2 units.
     __device__ __forceinline__ float put_query(uint32_t* to, float4 q, const float2& cs, const float2& sn) const {
         q = q4_rotate(q, cs, sn);
-        float back, bad = (q.x + q.y + q.z + q.w) * 0.0f;
+        float back, bad = fmaf(q.x, 0.0f, fmaf(q.y, 0.0f, fmaf(q.z, 0.0f, q.w * 0.0f)));
         const float mul = fixed_of(warp_max(fmaxf(fmaxf(fabsf(q.x), fabsf(q.y)), fmaxf(fabsf(q.z), fabsf(q.w)))), back);
         bad = __any_sync(0xffffffffu, bad != bad) ? __int_as_float(0x7fc00000) : 0.0f;      // NaN where the query holds an infinity or a NaN
         const uint32_t u0 = digits_of(q.x, mul), u1 = digits_of(q.y, mul), u2 = digits_of(q.z, mul), u3 = digits_of(q.w, mul);

@@ -184,21 +184,21 @@ __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int
             cs[h] = *reinterpret_cast<const float2*>(p.cosT + tab + 8 * h);      // the heads of a token share them: through L1
             sn[h] = *reinterpret_cast<const float2*>(p.sinT + tab + 8 * h);
         }
-        float most = 0.0f, all = 0.0f;
+        float most = 0.0f, none = 0.0f;           // none: NaN where a value is an infinity or a NaN
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             y[h] = q4_rotate(y[h], cs[h], sn[h]);
             most = fmaxf(most, q4_most(y[h]));
-            all += (y[h].x + y[h].y) + (y[h].z + y[h].w);
+            none = fmaf(y[h].x, 0.0f, fmaf(y[h].y, 0.0f, fmaf(y[h].z, 0.0f, fmaf(y[h].w, 0.0f, none))));
         }
-        if (all * 0.0f != 0.0f) most = INFINITY;
+        if (none != none) most = INFINITY;
 #pragma unroll
         for (int o = 1; o < LPR; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         // the largest value comes to 256 … 512
         most = fmaxf(most, 7.8886091e-31f);
         const int bits = __float_as_int(most) & 0x7f800000;
-        const bool fine = most < 1e30f;
-        const float mul = __int_as_float(0x7f000000 - bits) * 256.0f;
+        const bool fine = most < INFINITY;
+        const float mul = __uint_as_float((262u << 23) - (uint32_t)bits);        // 2^(8 - exponent): a normal number for every finite row
         uint4 h = make_uint4(0, 0, 0, 0), l = h;
         if (fine && on) {
             split_half(y[0].x * mul, y[0].z * mul, h.x, l.x);

@@ -1,5 +1,5 @@
 """Attention over the 4-bit cache where the numbers are far apart or add up: a key that takes nearly all of the weight above thousands that share the rest,
-sums of thousands of equal weights."""
+sums of thousands of equal weights, queries of any finite size."""
 import ctypes
 
 import numpy as np
@@ -88,3 +88,19 @@ def test_sums_of_equal_weights(dev, packed, G, n, nats):  # noqa: F811
     assert np.all(np.abs(got / 7.0 - 1.0) <= relative(score)), float(np.abs(got / 7.0 - 1.0).max() / relative(score))
     rest = (n + M - 1) * np.exp(-score)
     assert np.all(np.abs(weights[:, 1:] * (1.0 + rest) * np.exp(score) - 1.0) <= relative(score)), float(np.abs(weights[:, 1:] * (1.0 + rest) * np.exp(score) - 1.0).max())
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("value", [1e30, 1e32, 3e38])
+@pytest.mark.parametrize("hd,G,n", [(32, 2, 100), (64, 1, 3000), (128, 3, 70)])
+def test_large_queries_against_keys_of_zero(dev, packed, hd, G, n, value):  # noqa: F811
+    rng = np.random.default_rng(hd)
+    M = 5 if packed else 1
+    K, V, qkv = np.zeros((G, n, hd), np.float32), rows(rng, G, n, hd), rows(rng, M, 3 * G * hd)
+    qkv[:, :G * hd] = np.clip(qkv[:, :G * hd], -1, 1) * np.float32(value)
+    qkv[:, G * hd:2 * G * hd] = 0.0
+    got, _ = attend(dev, K, V, qkv, n, packed)
+    old, new = ref.stored(V).astype(np.float64), ref.stored(qkv[:, 2 * G * hd:]).reshape(M, G, hd).astype(np.float64)
+    for t in range(M):
+        want = (old.sum(1) + new[:t + 1].sum(0)) / (n + t + 1)
+        assert np.all(np.abs(got[t] - want) <= 2.0 ** -20 * np.abs(V).max() + 1e-12)
