@@ -53,6 +53,8 @@ constexpr int kSegment = 16;
 // fp16 end at 2^-24: with the maximum at 2^9, a weight is off by at most 2^-33 of the row's largest (two halves, half a step each).  With the maximum at 1, weights under
 // 2^-14 of it kept 10 bits and fewer, those under 2^-25 none: thousands of keys 10 … 18 nats below one were off by up to all of their sum.
 constexpr float kLift = 9.0f, kTop = 15.0f;
+// The base for a maximum; scores beyond 2^26 have no places for the lift, and a step of theirs may be more than it.
+__device__ __forceinline__ float base_of(float most) { return most - (most - kLift) > kTop ? most : most - kLift; }
 
 constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
 template <int NB> struct PrefillShape {
@@ -161,7 +163,8 @@ __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, i
 
 // Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 4·NB lanes of eight values each, one 16-byte piece;
 // `place(row, m, head, position)` says which one row `row` of the first `rows` is, and whether it is one (false: zeros, but the place can be read).
-// factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).  Bound by instructions: four values to a lane
+// factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).  It is a power of two, 1/sqrt(hd) · log2(e) goes
+// into the values: a score is then exact, and the one that its row's base was taken from comes to the lift again, however large scores are.  Bound by instructions: four values to a lane
 // took 12000 cycles a tile of four heads a token, eight 9000.  Loads of several rows ahead cost more in code than they give: the roles of a block share
 // the instruction cache (eight prompts of 1500: 303 µs as it is, 307 and 319 with two and three rows ahead).
 template <int NB, typename Place>
@@ -188,6 +191,7 @@ __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             y[h] = q4_rotate(y[h], cs[h], sn[h]);
+            y[h] = make_float4(y[h].x * p.scale, y[h].y * p.scale, y[h].z * p.scale, y[h].w * p.scale);
             most = fmaxf(most, q4_most(y[h]));
             none = fmaf(y[h].x, 0.0f, fmaf(y[h].y, 0.0f, fmaf(y[h].z, 0.0f, fmaf(y[h].w, 0.0f, none))));
         }
@@ -209,7 +213,7 @@ __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int
         const int to = at + r * 128 + (((c & 7) ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(hi + to) = h;
         *reinterpret_cast<uint4*>(lo + to) = l;
-        if (c == 0) factors[r] = fine || !on ? __int_as_float(bits) * (1.0f / 256.0f) * p.scale : __int_as_float(0x7fc00000);
+        if (c == 0) factors[r] = fine || !on ? __int_as_float(bits) * (1.0f / 256.0f) : __int_as_float(0x7fc00000);
     }
 }
 
@@ -446,9 +450,9 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 most = fmaxf(m2[0], m2[1]);
             }
             most *= c;
-            const bool grown = most > top + kTop;                        // also the first keys of a row
+            const bool grown = most - top > kTop;                        // also the first keys of a row
             if (__any_sync(0xffffffffu, grown)) {
-                const float now = grown ? most - kLift : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
+                const float now = grown ? base_of(most) : top, f = grown && top > -INFINITY ? ex2(top - now) : 1.0f;
                 if (j % kSegment > 0) {
                     if (!__all_sync(0xffffffffu, mbar_wait_long(vEmpty, (j - 1) & 1, &s_abort, p.error, 342))) ok = false;
                     tc_fence_after();

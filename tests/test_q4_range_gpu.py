@@ -1,5 +1,5 @@
-"""Attention over the 4-bit cache where the numbers are far apart or add up: a key that takes nearly all of the weight above thousands that share the rest,
-sums of thousands of equal weights, queries of any finite size."""
+"""Attention over the 4-bit cache where the numbers are far apart: a key that takes nearly all of the weight above thousands that share the rest, sums of
+thousands of equal weights, queries and scores of any finite size."""
 import ctypes
 
 import numpy as np
@@ -104,3 +104,29 @@ def test_large_queries_against_keys_of_zero(dev, packed, hd, G, n, value):  # no
     for t in range(M):
         want = (old.sum(1) + new[:t + 1].sum(0)) / (n + t + 1)
         assert np.all(np.abs(got[t] - want) <= 2.0 ** -20 * np.abs(V).max() + 1e-12)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("scale", [1e4, 1e7, 1e9, 1e12, 1e20])
+@pytest.mark.parametrize("hd,G,n", [(64, 2, 300), (128, 1, 3000)])
+def test_scores_of_any_size_choose_a_key(dev, packed, hd, G, n, scale):  # noqa: F811
+    """Scores so far apart that one weight is left: the output is that key's value, whatever the scores' size."""
+    rng = np.random.default_rng(hd + n)
+    M = 4 if packed else 1
+    K, V, qkv = rows(rng, G, n, hd), rows(rng, G, n, hd), rows(rng, M, 3 * G * hd)
+    qkv[:, :G * hd] *= np.float32(scale)
+    got, weights = attend(dev, K, V, qkv, n, packed, window=M)
+    assert np.all(np.abs(weights.astype(np.float64).sum(1) / M - 1.0) <= 2.0 ** -18)         # every token's weights add up to one
+    k64, v64 = ref.stored(K).astype(np.float64), ref.stored(V).astype(np.float64)
+    new = qkv.reshape(M, 3, G, hd)
+    for t in range(M):
+        for g in range(G):
+            k = np.concatenate((k64[g], ref.stored(new[:t + 1, 1, g]).astype(np.float64)))
+            v = np.concatenate((v64[g], ref.stored(new[:t + 1, 2, g]).astype(np.float64)))
+            q = new[t, 0, g].astype(np.float64)
+            sc, A = k @ q / np.sqrt(hd), (np.abs(k) @ np.abs(q) / np.sqrt(hd)).max()
+            order = np.argsort(sc)
+            gap = sc[order[-1]] - sc[order[-2]]
+            if gap < 30.0 + 4 * 2.0 ** -21 * A:                      # two keys the operands' 22 bits do not tell apart
+                continue
+            assert np.all(np.abs(got[t, g] - v[order[-1]]) <= 2.0 ** -20 * np.abs(v).max()), (t, g, got[t, g][:4], v[order[-1]][:4])
