@@ -194,7 +194,8 @@ struct Ctx {
     size_t ws_need = 0;
     int prev_op = 0;                   // op code before this one in the stream
     const int32_t* prev = nullptr;     // and its words
-    const int32_t* solid = nullptr;    // words of the last op before this one that is no Q8 projection
+    const int32_t* solid = nullptr;    // words of the last op before this one that launched something and is no Q8 projection
+    long long launches = 0;            // of the library when the op before this one began
     int next_op = 0;                   // op code behind this one, 0 = none
     bool bounded_waits = false;        // the stream holds an op whose kernel waits on a peer (tensor-parallel exchange)
     std::vector<std::pair<int, unsigned long long>>* refs = nullptr;
@@ -337,12 +338,14 @@ void do_op(Ctx& ctx, const int32_t* c) {
     // A projection lets the kernel behind it in before its own wait where that one reads nothing but weights ahead of its wait
     // (every older kernel may still run then, so nothing that keeps a state or a cache).
     const bool trigger = ctx.next_op == DEEPJ_OP_BF16_LINEAR || ctx.next_op == DEEPJ_OP_BF16_LINEAR_SUM || ctx.next_op == DEEPJ_OP_NORM_ADD;
-    // Q8 projections let the kernel behind them in before their own wait.  Behind any other op of this stream everything older is complete, so a cache
-    // may be read ahead of the wait behind projections that follow one which does not write that cache.
-    const bool q8 = op == DEEPJ_OP_Q8_LINEAR || op == DEEPJ_OP_Q8_LINEAR_LN || op == DEEPJ_OP_Q8_SWIGLU;
-    const int32_t* const solid = ctx.solid;
-    if (!q8) ctx.solid = c;
+    // Q8 projections let the kernel behind them in before their own wait.  Behind the kernels of any other op of this stream everything older is complete, so
+    // a cache may be read ahead of the wait behind projections that follow one which does not write that cache.  An op without work (a copy of nothing)
+    // has no kernel that waits: what is older may still run behind it.
     const int32_t* const prev = ctx.prev;
+    auto q8 = [](int o) { return o == DEEPJ_OP_Q8_LINEAR || o == DEEPJ_OP_Q8_LINEAR_LN || o == DEEPJ_OP_Q8_SWIGLU; };
+    if (prev != nullptr && !q8(prev[0]) && g_launches != ctx.launches) ctx.solid = prev;
+    ctx.launches = g_launches;
+    const int32_t* const solid = ctx.solid;
     ctx.prev_op = op; ctx.prev = c;
     auto scratch = [&](size_t floats) {          // room in the shared workspace for this op
         if (floats > ctx.ws_need) ctx.ws_need = floats;
