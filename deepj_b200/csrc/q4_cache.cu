@@ -23,13 +23,13 @@ struct AppendParams {
 __device__ __forceinline__ int sequence_of(const float* starts, int B, int M, int m, int lane, int& first, int& tokens) {
     for (int b0 = 0; b0 < B; b0 += 32) {
         const int b = b0 + lane;
-        int from = 0, to = 0;
-        if (b < B) { from = max(0, (int)starts[b]); to = min(M, (int)starts[b + 1]); }
-        const unsigned hit = __ballot_sync(0xffffffffu, b < B && m >= from && m < to);
+        int from = 0, n = 0;
+        if (b < B) n = q4_rows(starts[b], starts[b + 1], M, from);
+        const unsigned hit = __ballot_sync(0xffffffffu, m >= from && m - from < n);
         if (hit) {
             const int l = __ffs(hit) - 1;
             first = __shfl_sync(0xffffffffu, from, l);
-            tokens = __shfl_sync(0xffffffffu, to, l) - first;
+            tokens = __shfl_sync(0xffffffffu, n, l);
             return b0 + l;
         }
     }
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
         b = m / p.T;
         first = b * p.T;
     }
-    const int t = m - first, len = (int)p.len[b], pos = p.pos != nullptr ? (int)p.pos[b] : 0;
+    const int t = m - first, len = q4_int(p.len[b]), pos = p.pos != nullptr ? q4_int(p.pos[b]) : 0;
     if (t >= q4_room(tokens, len, p.maxSeq, pos, p.pos != nullptr ? p.maxPos : 0x7fffffff)) return;
     const int row = len + t, f = lane % LPR, at0 = (f >> 2) * 32 + (f & 3) * 4;      // this lane's values: at0 … at0 + 3, and 16 on
     const float* src = p.src + (size_t)m * p.ld;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) k_q4_load(const LoadParams p) {
     pdl_wait();
     pdl_launch_dependents();
     const int e = threadIdx.x % LPR, bg = blockIdx.y, b = bg / p.G;
-    const int at = p.at != nullptr ? (int)p.at[b] : 0, end = min(p.maxSeq, p.end != nullptr ? (int)p.end[b] : p.maxSeq);
+    const int at = p.at != nullptr ? q4_int(p.at[b]) : 0, end = min(p.maxSeq, p.end != nullptr ? q4_int(p.end[b]) : p.maxSeq);
     if (at < 0) return;
     const int j = e >> 2, t = e & 3;
     const unsigned char* const plane = p.cache + (size_t)bg * p.pages * Q4Page<NB>::kBytes;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kEvictThreads) k_q4_select(const EvictParams p
     pdl_launch_dependents();
     const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t bg = (size_t)b * p.G + g;
-    const int n = min(max((int)p.len[b], 0), p.srcMax), stay = min(n, p.budget), recent = min(p.recent, stay), top = stay - recent, old = n - recent;
+    const int n = min(max(q4_int(p.len[b]), 0), p.srcMax), stay = min(n, p.budget), recent = min(p.recent, stay), top = stay - recent, old = n - recent;
     const float* const acc = p.acc + bg * p.srcMax;
     int* const list = p.list + bg * p.budget;
     auto before = [&](int mine, int& total) {            // sum over the threads before this one, and over all
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(256) k_q4_move(const MoveParams p) {
     pdl_launch_dependents();
     const int g = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, t = lane & 3;
     const size_t bg = (size_t)b * p.G + g;
-    const int n = min(max((int)p.len[b], 0), p.srcMax), stay = min(n, p.budget);
+    const int n = min(max(q4_int(p.len[b]), 0), p.srcMax), stay = min(n, p.budget);
     if (p.inPlace && n <= p.budget) return;
     for (int to = (int)(blockIdx.x * 8 + (threadIdx.x >> 5)) * 8 + (lane >> 2); to < stay; to += gridDim.x * 64) {
         const int from = p.list != nullptr ? p.list[bg * p.budget + to] : to, rf = from % kQ4Page, rt = to % kQ4Page;

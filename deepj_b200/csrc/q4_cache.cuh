@@ -26,6 +26,13 @@ template <int NB> struct Q4Page {
     static __device__ __forceinline__ int word(int row, int t, int j) { return row * kRow + (t ^ ((row >> 1) & 3)) * (4 * NB) + 4 * j; }
 };
 
+// A length, position or place, which travel as floats: -1 for what is below 0 or no number, so that differences of two never leave 32 bits.
+__device__ __forceinline__ int q4_int(float x) { return x >= 0.0f ? (int)x : -1; }
+// Rows starts[b] … starts[b + 1] - 1 of the M packed rows: the first one, and how many.
+__device__ __forceinline__ int q4_rows(float start, float next, int M, int& first) {
+    first = min(max(q4_int(start), 0), M);
+    return max(0, min(q4_int(next), M) - first);
+}
 // Rows that a sequence has room for and positions that its tables have, of `tokens` new ones: 0 for a length or position outside its range.
 __device__ __forceinline__ int q4_room(int tokens, int len, int maxSeq, int pos, int maxPos) {
     if (len < 0 || len >= maxSeq || pos < 0 || pos >= maxPos) return 0;

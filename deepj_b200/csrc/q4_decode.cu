@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kShort) 
     int len = 0, pos = 0, first = 0, end = 0;
     bool there = false;
     auto place = [&]() {                          // where this sequence stands
-        len = (int)__ldcg(p.len + b); pos = (int)__ldcg(p.pos + b);
+        len = q4_int(__ldcg(p.len + b)); pos = q4_int(__ldcg(p.pos + b));
         there = q4_room(1, len, p.maxSeq, pos, p.maxPos) == 1;
         const int pages = len / kQ4Page + 1, share = (pages + splits - 1) / splits;
         first = min(pages, split * share);
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kShort) 
 // page took twice as long as all others.)
 constexpr int kHeadUnits = 4;
 __device__ __forceinline__ int pages_of(const DecodeParams& p, int b, int& len, int& pos) {
-    len = (int)p.len[b]; pos = (int)p.pos[b];
+    len = q4_int(p.len[b]); pos = q4_int(p.pos[b]);
     return q4_room(1, len, p.maxSeq, pos, p.maxPos) == 1 ? len / kQ4Page + 1 : 0;
 }
 __device__ __forceinline__ long long units_of(int pages, int heads) { return pages > 0 ? (long long)(pages + kHeadUnits) * heads : 0; }
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(256) k_q4_finish(const FinishParams p) {
     __shared__ float4 s_sum[8][32];
     pdl_wait();
     pdl_launch_dependents();
-    const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, len = (int)p.len[b], pos = (int)p.pos[b];
+    const int g = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, len = q4_int(p.len[b]), pos = q4_int(p.pos[b]);
     if (q4_room(1, len, p.maxSeq, pos, p.maxPos) != 1) return;
     const bool merges = (int)blockIdx.x < p.ratio;
     const int from = merges ? 0 : ((int)blockIdx.x - p.ratio) * kFinishRows, rec = p.hd + 2;

@@ -261,9 +261,8 @@ __device__ __forceinline__ bool tile_of(const PrefillParams& p, int tile, int to
     for (int b0 = 0; b0 < p.B; b0 += 32) {
         int from = 0, n = 0, l = 0, q = 0;
         if (b0 + lane < p.B) {
-            from = max(0, (int)__ldcg(p.starts + b0 + lane));
-            n = max(0, min(p.M, (int)__ldcg(p.starts + b0 + lane + 1)) - from);
-            l = (int)__ldcg(p.len + b0 + lane); q = (int)__ldcg(p.pos + b0 + lane);
+            n = q4_rows(__ldcg(p.starts + b0 + lane), __ldcg(p.starts + b0 + lane + 1), p.M, from);
+            l = q4_int(__ldcg(p.len + b0 + lane)); q = q4_int(__ldcg(p.pos + b0 + lane));
         }
         const int tiles = (n + tokensPerTile - 1) / tokensPerTile;
         int upto = tiles;
@@ -710,7 +709,8 @@ __global__ void __launch_bounds__(kWThreads, 2) k_q4_window(const PrefillParams 
         waited = true;
     };
     if (p.M == 0) wait();                         // there is no such kernel then
-    const int first = max(0, (int)__ldcg(p.starts + b)), tokens = max(0, min(p.M, (int)__ldcg(p.starts + b + 1)) - first), len = (int)__ldcg(p.len + b), pos = (int)__ldcg(p.pos + b);
+    int first;
+    const int tokens = q4_rows(__ldcg(p.starts + b), __ldcg(p.starts + b + 1), p.M, first), len = q4_int(__ldcg(p.len + b)), pos = q4_int(__ldcg(p.pos + b));
     const bool there = len >= 0 && len < p.maxSeq && pos >= 0 && pos < p.maxPos;
     const int room = q4_room(tokens, len, p.maxSeq, pos, p.maxPos), keys = there ? len + room : 0, pages = (keys + kQ4Page - 1) / kQ4Page;
     const int window = min(p.window, room), rows = window * p.ratio;

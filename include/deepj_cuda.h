@@ -310,8 +310,8 @@ int deepj_cuda_latent_alloc(int32_t id, int32_t batch, int32_t max_seq, int32_t 
  *                        position 0 starts from zeros (csrc/mlstm.cu)
  *
  * Ops over a 4-bit cache (deepj_cuda_kv_alloc_q4), H query heads over its G key/value heads, H a multiple of G.  A sequence whose length is
- * outside 0 … max_seq - 1 or whose position is outside 0 … max_pos - 1 is left out: nothing of it is appended or written.  Tokens that
- * do not fit (behind max_seq rows or max_pos positions) are left out as well.  Offsets and strides are multiples of four floats.
+ * outside 0 … max_seq - 1 or whose position is outside 0 … max_pos - 1 (NaN is) is left out: nothing of it is appended or written.  Tokens that
+ * do not fit (behind max_seq rows or max_pos positions) are left out as well, rows outside 0 … M - 1 are none of a sequence's.  Offsets and strides are multiples of four floats.
  *
  *  87 ATTN_DECODE_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, acc, acc_out]
  *                        one token of every sequence: q and k rotated at pos[b] (tables [max_pos][hd/2]), k and v appended as row len[b], softmax
