@@ -10,6 +10,7 @@
 #include "q8_tma.cuh"
 
 #include <deque>
+#include <initializer_list>
 #include <iterator>
 #include <list>
 #include <algorithm>
@@ -319,6 +320,10 @@ int op_stride(int op) {
 
 inline size_t sz(int a, int b) { return (size_t)a * (size_t)b; }
 
+// Blocks and kernels of one op read their inputs at different times: a buffer it writes is none of these (ids below 0: none).
+void apart(int out, std::initializer_list<int> others, const char* what) {
+    for (int id : others) require(out < 0 || id != out, what, "an output goes to another buffer than the inputs and the other outputs");
+}
 // A layer of a 4-bit cache that at least B sequences fit into.
 unsigned char* q4_layer(const Buf& kv, int B, int layer, const char* what) {
     require(B >= 1 && B <= kv.B, what, "batch does not match the cache");
@@ -767,6 +772,8 @@ void do_op(Ctx& ctx, const int32_t* c) {
             a.cosT = f32(ctx, e[10], sz(a.maxPos, a.hd / 2), what); a.sinT = f32(ctx, e[11], sz(a.maxPos, a.hd / 2), what);
             a.out = f32(ctx, e[13], a.M ? (size_t)e[14] + sz(last, a.ldo) + a.H * a.hd : 0, what) + e[14];
             require(a.M == 0 || e[13] != c[1], what, "the output goes to another buffer than the rows");
+            if (a.M > 0) apart(e[13], {packed ? c[8] : -1, e[8], e[9], e[10], e[11], w[0], w[1]}, what);
+            apart(w[1], {c[1], packed ? c[8] : -1, e[8], e[9], e[10], e[11]}, what);
             require((w[0] < 0) == (w[1] < 0), what, "accumulated weights need both an input and an output (which may be the same buffer)");
             require(!packed || (w[0] < 0) == (a.window == 0), what, "a window goes with accumulated weights, and they with a window");
             a.acc = f32_opt(ctx, w[0], sz(a.B, a.G) * a.maxSeq, what); a.accOut = f32_opt(ctx, w[1], sz(a.B, a.G) * a.maxSeq, what);
@@ -787,6 +794,9 @@ void do_op(Ctx& ctx, const int32_t* c) {
             require(a.budget >= 1 && a.budget <= dst.maxSeq && a.recent >= 0 && a.recent <= a.budget, what, "bad budget or number of recent rows");
             require(a.B <= 65535, what, "too many sequences");
             require(c[10] != c[4], what, "the lengths go to another buffer than they come from");
+            apart(c[9], {c[4], c[10], c[11]}, what);
+            apart(c[10], {c[5], c[11]}, what);
+            apart(c[11], {c[4], c[5]}, what);
             require(c[9] != c[5] || a.srcMax == a.dstMax, what, "weights that stay in place need caches of one size");
             a.len = f32(ctx, c[4], a.B, what);
             a.acc = f32(ctx, c[5], sz(a.B, a.G) * a.srcMax, what); a.accOut = f32(ctx, c[9], sz(a.B, a.G) * a.dstMax, what);
@@ -819,6 +829,8 @@ void do_op(Ctx& ctx, const int32_t* c) {
             a.B = c[8]; a.G = kv.H; a.hd = kv.hd; a.maxSeq = kv.maxSeq; a.T = c[5];
             a.cache = q4_layer(kv, a.B, c[2], what);
             require(a.T >= 0 && sz(a.B, a.G) <= 65535, what, "bad number of rows or heads");
+            apart(c[6], {c[3], c[4]}, what);
+            apart(c[7], {c[3], c[4]}, what);
             a.at = f32_opt(ctx, c[3], a.B, what); a.end = f32_opt(ctx, c[4], a.B, what);
             a.k = f32(ctx, c[6], sz(a.B, a.G) * a.T * a.hd, what); a.v = f32(ctx, c[7], sz(a.B, a.G) * a.T * a.hd, what);
             if (go) launch_q4_load(a, s);

@@ -63,3 +63,63 @@ def test_a_step_waits_for_the_op_that_writes_its_rows(box, writer):  # noqa: F81
         assert t.early(*w, *t.q8, *idle, *t.step()) == 0
         t.box.flush(*w)
         assert t.early(*idle, *t.q8, *t.step()) == 0                 # nor when the writer ran in the stream before
+
+
+# ───────────── outputs among the inputs ─────────────
+
+def refused(box, words, at, value, match="another buffer"):  # noqa: F811
+    words = list(words)
+    words[at] = value
+    box.launched()
+    with pytest.raises(RuntimeError, match=match):
+        box.flush(*words)
+    assert box.launched() == []
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_attention_writes_to_none_of_its_inputs(box, packed):  # noqa: F811
+    t = Step(box)
+    words, e = (t.writers()["packed"], 1) if packed else (t.step(), 0)
+    old, new, pos = box.zeros(128), box.zeros(128), box.zeros(4)
+    words[9 + e], words[11 + e] = pos, box.zeros(64 * 16)            # every input a buffer of its own
+    words[-3:] = [old, new, 1] if packed else words[-3:-2] + [old, new]
+    box.flush(*words)
+    acc, acc_out = (20, 21) if packed else (18, 19)
+    inputs = [1] + ([8] if packed else []) + [8 + e, 9 + e, 10 + e, 11 + e]
+    big = {i: box.zeros(64 * 16) for i in inputs}                    # large enough for what is written
+    for i in inputs:
+        words[i] = big[i]
+    box.flush(*words)
+    for i in inputs:
+        refused(box, words, 13 + e, big[i])
+        refused(box, words, acc_out, big[i])
+    refused(box, words, 13 + e, old)
+    refused(box, words, 13 + e, new)
+    refused(box, words, acc_out, words[13 + e])
+    words[acc_out] = old                                             # added up in place
+    box.flush(*words)
+    assert acc == acc_out - 1 and words[acc] == old
+
+
+def test_eviction_writes_to_none_of_its_inputs(box):  # noqa: F811
+    kv, small = box.cache(1, 2, 1, 64, 32), box.cache(1, 2, 1, 16, 32)
+    n, acc, new, n_out, kept = (box.zeros(512) for _ in range(5))
+    words = [cg.OP_KV_EVICT_Q4, kv, small, 0, n, acc, 8, 2, 2, new, n_out, kept]
+    box.flush(*words)
+    for at, others in ((9, (n, n_out, kept)), (10, (n, acc, new, kept)), (11, (n, acc, new, n_out))):
+        for other in others:
+            refused(box, words, at, other)
+    words[2], words[9] = kv, acc                                     # in place
+    box.flush(*words)
+
+
+def test_a_row_load_writes_to_none_of_its_inputs(box):  # noqa: F811
+    kv = box.cache(1, 2, 1, 64, 32)
+    at, end, k, v = (box.zeros(512) for _ in range(4))
+    words = [cg.OP_KV_LOAD_Q4, kv, 0, at, end, 4, k, v, 2]
+    box.flush(*words)
+    for slot in (6, 7):
+        refused(box, words, slot, at)
+        refused(box, words, slot, end)
+    words[3] = words[4] = -1
+    box.flush(*words)
