@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(256) k_q4_append(const AppendParams p) {
 // Values of rows at[b] … of every head → [B][G][T][hd], as far as end[b]; other rows of the outputs stay as they are.
 struct LoadParams {
     const unsigned char* cache; int maxSeq, pages;
-    const float* at; const float* end; float* k; float* v; int B, G, T;
+    const float* at; const float* end; float* k; float* v; int B, G, T, share;      // share: blocks of a head
 };
 // A lane takes a word: four values and the four 16 on.  Bound by the writes (16 × 32 heads × 1024 rows of 128: 100 µs for 613 MB in and out; 104 with a
 // lane to four values).
@@ -104,15 +104,15 @@ __global__ void __launch_bounds__(256) k_q4_load(const LoadParams p) {
     constexpr int LPR = 4 * NB, AHEAD = 4;               // lanes of a row; rows whose loads go out together
     pdl_wait();
     pdl_launch_dependents();
-    const int e = threadIdx.x % LPR, bg = blockIdx.y, b = bg / p.G;
+    const int e = threadIdx.x % LPR, bg = blockIdx.x / p.share, b = bg / p.G;
     const int at = p.at != nullptr ? q4_int(p.at[b]) : 0, end = min(p.maxSeq, p.end != nullptr ? q4_int(p.end[b]) : p.maxSeq);
     if (at < 0) return;
     const int j = e >> 2, t = e & 3;
     const unsigned char* const plane = p.cache + (size_t)bg * p.pages * Q4Page<NB>::kBytes;
     const size_t out = (size_t)bg * p.T * (32 * NB) + 32 * j + 4 * t;
-    const int rows = min(p.T, end - at), step = gridDim.x * (256 / LPR);
+    const int rows = min(p.T, end - at), step = p.share * (256 / LPR);
 #pragma unroll 1
-    for (int i0 = blockIdx.x * (256 / LPR) + threadIdx.x / LPR; i0 < rows; i0 += AHEAD * step) {
+    for (int i0 = ((int)blockIdx.x - bg * p.share) * (256 / LPR) + threadIdx.x / LPR; i0 < rows; i0 += AHEAD * step) {
         uint32_t w[AHEAD][2];
         unsigned short scale[AHEAD][2];
 #pragma unroll
@@ -301,9 +301,10 @@ __global__ void __launch_bounds__(256) k_q4_move(const MoveParams p) {
 }
 
 template <int NB> void append(const AppendParams& p, cudaStream_t s) { launch_k(k_q4_append<NB>, dim3((unsigned)(((long long)p.M * p.share + 7) / 8)), dim3(256), 0, s, true, p); }
-template <int NB> void load(const LoadParams& p, cudaStream_t s) {
-    const int per = 256 / (4 * NB), blocks = std::min((p.T + per - 1) / per, std::max(1, 16 * g_num_sms / (p.B * p.G)));
-    launch_k(k_q4_load<NB>, dim3(blocks, p.B * p.G), dim3(256), 0, s, true, p);
+template <int NB> void load(LoadParams p, cudaStream_t s) {
+    const int per = 256 / (4 * NB);
+    p.share = std::min((p.T + per - 1) / per, std::max(1, 16 * g_num_sms / (p.B * p.G)));
+    launch_k(k_q4_load<NB>, dim3((unsigned)(p.share * p.B * p.G)), dim3(256), 0, s, true, p);
 }
 template <int NB> void move(const MoveParams& p, int B, cudaStream_t s) {
     const int most = std::max(1, 8 * 8 * g_num_sms / (p.G * B));         // blocks of a head: all heads' fill the chip some times over
@@ -326,7 +327,7 @@ void launch_q4_append(const Q4AttnArgs& a, int T, cudaStream_t s) {
 }
 void launch_q4_load(const Q4LoadArgs& a, cudaStream_t s) {
     if (a.T == 0) return;
-    LoadParams p = {a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.at, a.end, a.k, a.v, a.B, a.G, a.T};
+    LoadParams p = {a.cache, a.maxSeq, (a.maxSeq + kQ4Page - 1) / kQ4Page, a.at, a.end, a.k, a.v, a.B, a.G, a.T, 1};
     if (a.hd == 128) load<4>(p, s); else if (a.hd == 64) load<2>(p, s); else load<1>(p, s);
 }
 // In place: the rows that stay, in pages as well.  The list of rows follows.

@@ -828,7 +828,7 @@ void do_op(Ctx& ctx, const int32_t* c) {
             Q4LoadArgs a = {};
             a.B = c[8]; a.G = kv.H; a.hd = kv.hd; a.maxSeq = kv.maxSeq; a.T = c[5];
             a.cache = q4_layer(kv, a.B, c[2], what);
-            require(a.T >= 0 && sz(a.B, a.G) <= 65535, what, "bad number of rows or heads");
+            require(a.T >= 0, what, "bad number of rows");
             apart(c[6], {c[3], c[4]}, what);
             apart(c[7], {c[3], c[4]}, what);
             a.at = f32_opt(ctx, c[3], a.B, what); a.end = f32_opt(ctx, c[4], a.B, what);

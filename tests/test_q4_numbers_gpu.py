@@ -1,7 +1,9 @@
-"""Lengths, positions and places of the 4-bit cache's ops that are no numbers, or far outside: sequences that are left out, never rows that are not there."""
+"""Lengths, positions and places of the 4-bit cache's ops that are no numbers, or far outside: sequences that are left out, never rows that are not there.  As many
+sequences times heads as there may be."""
 import numpy as np
 import pytest
 
+import q4_ref as ref
 from deepj_b200 import compute_graph as cg
 from test_q4_cache_gpu import FILL, dev, rows, tables  # noqa: F401
 
@@ -94,3 +96,18 @@ def test_eviction(dev):  # noqa: F811
     k, _ = dev.load(small, 0, B, G, budget, HD)
     for b, x in enumerate(OUT):
         assert np.any(k[b]) == (x > 0)
+
+
+def test_rows_of_as_many_heads_as_a_cache_has(dev):  # noqa: F811
+    """More than 65535 sequences times heads: stored, loaded, moved."""
+    B, heads, rows_of = 2060, 32, 2
+    k, v = (np.random.default_rng(6 + i).standard_normal((B, heads, rows_of, HD)).astype(np.float32) for i in range(2))
+    kv, other = dev.cache(1, B, heads, rows_of, HD), dev.cache(1, B, heads, 1, HD)
+    dev.store(kv, 0, k, v)
+    gk, gv = dev.load(kv, 0, B, heads, rows_of, HD)
+    assert np.array_equal(gk, ref.stored(k)) and np.array_equal(gv, ref.stored(v))
+    w = np.random.default_rng(8).random((B, heads, rows_of)).astype(np.float32)
+    dev.flush(cg.OP_KV_EVICT_Q4, kv, other, 0, dev.buf(np.full(B, rows_of)), dev.buf(w), 1, 0, B, dev.buf(np.zeros(B * heads)), dev.buf(np.zeros(B)), -1)
+    ok, ov = dev.load(other, 0, B, heads, 1, HD)
+    at = w.argmax(2)[..., None, None]
+    assert np.array_equal(ok, np.take_along_axis(gk, at, 2)) and np.array_equal(ov, np.take_along_axis(gv, at, 2))
