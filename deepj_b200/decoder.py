@@ -627,10 +627,10 @@ class Q8Decoder(StreamDecoder):
             self._set_rows(np.zeros(self.B, dtype=np.int64))
 
     def set_position(self, position: int) -> None:
-        if self.kv_dtype == "q4" and position > self.kv_rows:
-            raise ValueError(f"position {position} outside the cache's {self.kv_rows} rows")
         if self.kv_dtype == "q4" and position != 0 and self._evicted:
             raise ValueError("rows have been evicted: reset() and feed the tokens again")
+        if self.kv_dtype == "q4" and position > int(self._rows.min()):       # packed prompts differ in length
+            raise ValueError(f"position {position} outside the {int(self._rows.min())} rows that every sequence has")
         super().set_position(position)
         if self.kv_dtype == "q4":
             self._set_rows(np.full(self.B, position, dtype=np.int64))

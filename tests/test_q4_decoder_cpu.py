@@ -1,0 +1,58 @@
+"""What a decoder over the 4-bit cache keeps about its sequences' rows, without a GPU: the interpreter over a stand-in for the kernels."""
+import numpy as np
+import pytest
+
+from deepj_b200 import compute_graph as cg
+from deepj_b200.decoder import DecoderConfig, Q8Decoder
+from q4_standin import box, standin  # noqa: F401
+
+CFG = DecoderConfig("gpt", 64, 96, 64, 2, 1, 96)
+
+
+@pytest.fixture
+def make(box):  # noqa: F811
+    made = []
+
+    def decoder(batch=1, **kw):
+        d = Q8Decoder(CFG, batch=batch, kv_dtype="q4", id_base=(1 << 24) + (len(made) << 16), **kw)
+        made.append(d)
+        d.load_synthetic(1, 0.05)
+        return d
+    yield decoder
+    for d in made:
+        d.close()
+
+
+def state(d):
+    """Rows as the host counts them, lengths and positions as the device holds them."""
+    return d._rows.tolist(), d._download(d.ids["len"], d.B).astype(int).tolist(), d._download(d.ids["pos"], d.B).astype(int).tolist()
+
+
+def test_rows_and_positions_follow_what_is_fed(make):
+    d = make(2)
+    d.prefill_packed([[1] * 5, [2] * 40])
+    assert state(d) == ([5, 40],) * 3
+    d.step([1, 2])
+    d.step_device(3)
+    assert state(d) == ([9, 44],) * 3 and d.position == 44
+    d.prefill([[1] * 33, [2] * 33])
+    assert state(d) == ([42, 77],) * 3
+    d.reset()
+    assert state(d) == ([0, 0],) * 3
+
+
+def test_no_sequence_is_set_to_rows_it_does_not_have(make):
+    d = make(2)
+    d.prefill_packed([[1] * 5, [2] * 40])
+    for position in (6, 40, 41):
+        with pytest.raises(ValueError, match="rows"):
+            d.set_position(position)
+    assert state(d) == ([5, 40],) * 3 and d.position == 40
+    d.set_position(5)
+    assert state(d) == ([5, 5],) * 3 and d.position == 5
+    d.step([1, 2])
+    d.set_position(6)
+    assert state(d) == ([6, 6],) * 3
+    d.set_position(0)
+    with pytest.raises(ValueError, match="rows"):
+        d.set_position(1)
