@@ -631,6 +631,8 @@ class Q8Decoder(StreamDecoder):
             raise ValueError("rows have been evicted: reset() and feed the tokens again")
         if self.kv_dtype == "q4" and position > int(self._rows.min()):       # packed prompts differ in length
             raise ValueError(f"position {position} outside the {int(self._rows.min())} rows that every sequence has")
+        if self.kv_dtype == "q4" and self.kv_budget is not None and position != 0 and np.any(self._rows != position):
+            raise ValueError("the attention that later tokens gave to cached rows stays with them: reset() and feed the tokens again")
         super().set_position(position)
         if self.kv_dtype == "q4":
             self._set_rows(np.full(self.B, position, dtype=np.int64))

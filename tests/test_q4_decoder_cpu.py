@@ -56,3 +56,16 @@ def test_no_sequence_is_set_to_rows_it_does_not_have(make):
     d.set_position(0)
     with pytest.raises(ValueError, match="rows"):
         d.set_position(1)
+
+
+def test_a_bounded_cache_is_not_set_back(make):
+    """The attention that rows got from tokens behind the position cannot be taken away again, and it decides what is evicted."""
+    d = make(2, kv_rows=64, kv_budget=40)
+    d.prefill([[1] * 20, [2] * 20])
+    for position in (1, 19):
+        with pytest.raises(ValueError, match="attention"):
+            d.set_position(position)
+    d.set_position(20)                                               # where it is
+    assert state(d) == ([20, 20],) * 3
+    d.set_position(0)
+    assert state(d) == ([0, 0],) * 3
