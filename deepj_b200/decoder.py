@@ -618,8 +618,7 @@ class Q8Decoder(StreamDecoder):
     # ── the 4-bit cache ──
     def _check_tokens(self, p: np.ndarray) -> None:
         super()._check_tokens(p)
-        if self.kv_dtype == "q4" and self.kv_budget is None and int(self._rows.max()) + p.shape[1] > self.kv_rows:
-            raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+        self._check_room(p.shape[1])
 
     def reset(self) -> None:
         super().reset()
@@ -644,14 +643,23 @@ class Q8Decoder(StreamDecoder):
 
     _evicted = False         # cached rows are no longer the first positions
 
-    def _take_rows(self, tokens) -> None:
-        """Room for `tokens` new rows (of every sequence, or one number each) in a 4-bit cache: evict where they would not fit, then count them."""
+    def _check_room(self, tokens) -> None:
+        """Refuses `tokens` new rows (of every sequence, or one number each) that a 4-bit cache without a budget has no room for."""
+        if self.kv_dtype == "q4" and self.kv_budget is None and np.any(self._rows + tokens > self.kv_rows):
+            raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+
+    def _advance(self, tokens) -> None:
+        super()._advance(int(np.max(tokens)))
+        if self.kv_dtype == "q4":
+            self._rows = self._rows + tokens
+
+    def _make_room(self, tokens) -> None:
+        """Room for `tokens` new rows (of every sequence, or one number each) in a 4-bit cache: evict where they would not fit."""
+        self._check_room(tokens)
         if self.kv_dtype != "q4":
             return
         need = np.broadcast_to(np.asarray(tokens, dtype=np.int64), (self.B,))
         if np.any(self._rows + need > self.kv_rows):
-            if self.kv_budget is None:
-                raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
             I, s = self.ids, []
             for l in range(self.cfg.n_layers):
                 seen = I[f"seen.{l}"]
@@ -662,7 +670,6 @@ class Q8Decoder(StreamDecoder):
             self._rows = np.minimum(self._rows, self.kv_budget)
             if np.any(self._rows + need > self.kv_rows):
                 raise ValueError("more tokens at once than the cache has rows behind its budget")
-        self._rows = self._rows + need
 
     def prefill_packed(self, prompts) -> np.ndarray:
         """Feed prompts of different lengths, one per sequence (each at least one token), behind whatever the sequences hold; returns the greedy
@@ -683,8 +690,7 @@ class Q8Decoder(StreamDecoder):
             if pos[b] + t.size > self.cfg.max_seq_len:
                 raise ValueError(f"seqLen {int(pos[b]) + t.size} exceeds maxSeqLen {self.cfg.max_seq_len}")
         longest = max(t.size for t in toks)
-        if self.kv_budget is None and any(self._rows[b] + t.size > self.kv_rows for b, t in enumerate(toks)):
-            raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+        self._check_room(np.asarray([t.size for t in toks]))
         C = min(self._chunk_tokens(), longest)
         self._ensure_prefill_buffers(C)
         P, I = self._prefill_ids, self.ids
@@ -693,17 +699,18 @@ class Q8Decoder(StreamDecoder):
             new = np.asarray([t.size for t in parts], dtype=np.int64)
             starts = np.concatenate(([0], np.cumsum(new)))
             ends = [(b, int(starts[b + 1]) - 1) for b in range(self.B) if new[b] > 0 and lo + C >= toks[b].size]
-            self._take_rows(new)
+            self._make_room(new)
             self._upload(P["tok"], np.concatenate(parts).astype(np.float32))
             self._upload(P["starts"], starts)
             if self.cfg.kind == "gpt":
                 self._upload(P["ppos"], np.concatenate([np.arange(pos[b], pos[b] + new[b]) for b in range(self.B)]))
             st = self._build_prefill(0, ends, int(starts[-1]))
             _lib.check(self.lib.deepj_cuda_flush_ops(st.ctypes.data, st.size))
+            self._advance(new)
             pos += new
+            self.position = int(pos.max())
             self._upload(I["pos"], pos.astype(np.float32))
             self._upload(I["len"], self._rows.astype(np.float32))
-        self.position = int(pos.max())
         hs = self._head_stream()
         _lib.check(self.lib.deepj_cuda_flush_ops(hs.ctypes.data, hs.size))
         return self.next_tokens()

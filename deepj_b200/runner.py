@@ -73,8 +73,15 @@ class StreamDecoder:
         """Token ids [B × T] of the next chunk (row b·T + t)."""
         self._upload(self._prefill_ids["tok"], tokens.astype(np.float32).reshape(-1))
 
-    def _take_rows(self, tokens: int) -> None:
-        """Called before `tokens` new tokens of every sequence run: a cache that fills up makes room here."""
+    def _check_room(self, tokens: int) -> None:
+        """Refuses `tokens` more tokens of every sequence where a cache cannot hold them."""
+
+    def _make_room(self, tokens: int) -> None:
+        """Called before `tokens` new tokens of every sequence run: a cache that is full makes room here."""
+
+    def _advance(self, tokens: int) -> None:
+        """Counts `tokens` tokens of every sequence, which have been enqueued."""
+        self.position += tokens
 
     # ── id / buffer helpers ──
     def _new_id(self) -> int:
@@ -165,10 +172,10 @@ class StreamDecoder:
             raise ValueError(f"seqLen {self.position + 1} exceeds maxSeqLen {self.cfg.max_seq_len}")
         host, _ = self._streams()
         self.set_tokens(tokens)
-        self._take_rows(1)
+        self._make_room(1)
         # enqueue the stream behind the upload and let the download's synchronisation be the only one of the step
         _lib.check(self.lib.deepj_cuda_flush_ops_async(host.ctypes.data, host.size))
-        self.position += 1
+        self._advance(1)
         _, nxt = self._pinned()
         _lib.check(self.lib.deepj_cuda_download_buffer(self.ids["next"], nxt.ctypes.data, self.B))
         return nxt.astype(np.int64)
@@ -178,10 +185,11 @@ class StreamDecoder:
         if self.position + n_steps > self.cfg.max_seq_len:
             raise ValueError(f"seqLen {self.position + n_steps} exceeds maxSeqLen {self.cfg.max_seq_len}")
         _, dev = self._streams()
+        self._check_room(n_steps)
         for _ in range(n_steps):
-            self._take_rows(1)
+            self._make_room(1)
             _lib.check(self.lib.deepj_cuda_flush_ops_async(dev.ctypes.data, dev.size))
-        self.position += n_steps
+            self._advance(1)
         if sync:
             _lib.check(self.lib.deepj_cuda_synchronize())
 
@@ -212,10 +220,10 @@ class StreamDecoder:
                 self._prefill_streams.clear()
             self._prefill_streams[T] = self._build_prefill(T)
         st = self._prefill_streams[T]
-        self._take_rows(T)
+        self._make_room(T)
         self._upload_chunk(p)
         _lib.check(self.lib.deepj_cuda_flush_ops(st.ctypes.data, st.size))
-        self.position += T
+        self._advance(T)
 
     def prefill(self, prompts, chunked: Optional[bool] = None) -> np.ndarray:
         """Feed the prompt (every sequence the same length) from the current position; returns the greedy pick after its
@@ -324,10 +332,10 @@ class StreamDecoder:
             else:
                 if self.position + 1 > c.max_seq_len:
                     raise ValueError(f"seqLen {self.position + 1} exceeds maxSeqLen {c.max_seq_len}")
-                self._take_rows(1)
+                self._make_room(1)
                 self._upload(I["tok"], np.asarray([out[-1]], dtype=np.float32))
                 _lib.check(self.lib.deepj_cuda_flush_ops(step.ctypes.data, step.size))
-                self.position += 1
+                self._advance(1)
             out.append(int(self.next_tokens()[0]))
         return np.asarray(out, dtype=np.int64)
 
@@ -357,12 +365,12 @@ class StreamDecoder:
         if not self.loaded:
             raise RuntimeError("weights are not loaded")
         host = self._build(feed_back=False)
-        self._take_rows(1)
+        self._make_room(1)
         n = len(self._op_labels) + 1
         ms = np.zeros(n, dtype=np.float32)
         cnt = ctypes.c_int32(0)
         _lib.check(self.lib.deepj_cuda_profile_ops(host.ctypes.data, host.size, ms.ctypes.data, n, ctypes.byref(cnt)))
-        self.position += 1
+        self._advance(1)
         return list(zip(self._op_labels, ms[: cnt.value].tolist()))
 
     def time_ops(self, labels, iters: int = 20, warmup: int = 3) -> Tuple[float, int]:

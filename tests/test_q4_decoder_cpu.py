@@ -69,3 +69,43 @@ def test_a_bounded_cache_is_not_set_back(make):
     assert state(d) == ([20, 20],) * 3
     d.set_position(0)
     assert state(d) == ([0, 0],) * 3
+
+
+def test_steps_that_do_not_fit_are_refused_before_the_first(make):
+    d = make(2, kv_rows=48)
+    d.prefill_packed([[1] * 40, [2] * 3])
+    with pytest.raises(ValueError, match="48 rows"):
+        d.step_device(9)
+    assert state(d) == ([40, 3],) * 3 and d.position == 40
+    d.step_device(8)
+    assert state(d) == ([48, 11],) * 3 and d.position == 48
+    with pytest.raises(ValueError, match="48 rows"):
+        d.step([1, 2])
+    assert state(d) == ([48, 11],) * 3
+
+
+def test_what_did_not_run_is_not_counted(make, monkeypatch):
+    """A flush that fails (no memory for the workspace, say) leaves rows and position as they were."""
+    d = make(1, kv_rows=64, kv_budget=40)
+    d.prefill([[1] * 33])
+
+    def fails(*_):
+        raise RuntimeError("out of memory")
+    for call in (lambda: d.step([1]), lambda: d.step_device(2), lambda: d.prefill([[1] * 20], chunked=True), lambda: d.prefill_packed([[1] * 20])):
+        d._streams()
+        d._ensure_prefill_buffers(24)
+        with monkeypatch.context() as m:
+            m.setattr(d, "lib", Failing(d.lib, fails))
+            with pytest.raises(RuntimeError, match="out of memory"):
+                call()
+        assert state(d) == ([33],) * 3 and d.position == 33
+
+
+class Failing:
+    """A library whose flushes fail."""
+
+    def __init__(self, lib, fails):
+        self._real, self.deepj_cuda_flush_ops, self.deepj_cuda_flush_ops_async = lib, fails, fails
+
+    def __getattr__(self, name):
+        return getattr(self._real, name)
