@@ -171,8 +171,9 @@ class Q8Decoder(StreamDecoder):
         `kv_dtype`: "f32" (the reference's precision) or "f16" — keys rounded after the rotation, values rounded, fp32
         arithmetic; half the bytes a step's attention reads — or "q4": 4-bit codes with a scale to 32 values, a seventh of the fp32 bytes,
         prompts of different lengths (`prefill_packed`).  `kv_rows` ("q4"): cached rows per sequence, at most `max_seq_len`, which is the
-        default.  `kv_budget`: a cache without room for the next tokens is cut to so many rows, the newest `kv_recent` (default: a quarter
-        of them) and those that got the most attention so far; without a budget a full cache is an error."""
+        default.  `kv_budget`: a sequence without room for its next tokens is cut to so many rows, the newest `kv_recent` (default: a quarter
+        of them) and those that got the most attention so far; prompts then run in chunks of at most `kv_rows` - `kv_budget` tokens, which fit
+        behind an eviction.  Without a budget a full sequence is an error."""
         if kv_dtype not in ("f32", "f16", "q4"):
             raise ValueError("kv_dtype must be 'f32', 'f16' or 'q4'")
         if kv_dtype != "q4" and (kv_rows, kv_budget, kv_recent) != (None, None, None):
@@ -265,6 +266,7 @@ class Q8Decoder(StreamDecoder):
             self._rows = np.zeros(B, dtype=np.int64)         # cached rows of every sequence: "len" on the device
             self._f32("len", B)
             if self.kv_budget is not None:
+                self._f32("len_full", B)
                 self._f32("len_kept", B)
                 for l in range(c.n_layers):
                     self._f32(f"seen.{l}", B * self.h_local * self.kv_rows)      # attention every cached row has got so far
@@ -654,22 +656,26 @@ class Q8Decoder(StreamDecoder):
             self._rows = self._rows + tokens
 
     def _make_room(self, tokens) -> None:
-        """Room for `tokens` new rows (of every sequence, or one number each) in a 4-bit cache: evict where they would not fit."""
+        """Room for `tokens` new rows (of every sequence, or one number each) in a 4-bit cache: the sequences where they would not fit are evicted from."""
         self._check_room(tokens)
         if self.kv_dtype != "q4":
             return
-        need = np.broadcast_to(np.asarray(tokens, dtype=np.int64), (self.B,))
-        if np.any(self._rows + need > self.kv_rows):
-            I, s = self.ids, []
-            for l in range(self.cfg.n_layers):
-                seen = I[f"seen.{l}"]
-                s += [OP_KV_EVICT_Q4, I["kv"], I["kv"], l, I["len"], seen, self.kv_budget, self.kv_recent, self.B, seen, I["len_kept"], -1]
-            s = np.asarray(s + [OP_COPY, I["len_kept"], 0, I["len"], 0, self.B], dtype=np.int32)
-            _lib.check(self.lib.deepj_cuda_flush_ops_async(s.ctypes.data, s.size))
-            self._evicted = self._evicted or bool(np.any(self._rows > self.kv_budget))
-            self._rows = np.minimum(self._rows, self.kv_budget)
-            if np.any(self._rows + need > self.kv_rows):
-                raise ValueError("more tokens at once than the cache has rows behind its budget")
+        full = self._rows + tokens > self.kv_rows
+        if not full.any():
+            return
+        kept = np.where(full, np.minimum(self._rows, self.kv_budget), self._rows)
+        if np.any(kept + tokens > self.kv_rows):
+            raise ValueError("more tokens at once than the cache has rows behind its budget")
+        I, s = self.ids, []
+        self._upload(I["len_full"], np.where(full, self._rows, 0))       # of sequences without rows nothing leaves or moves
+        for l in range(self.cfg.n_layers):
+            seen = I[f"seen.{l}"]
+            s += [OP_KV_EVICT_Q4, I["kv"], I["kv"], l, I["len_full"], seen, self.kv_budget, self.kv_recent, self.B, seen, I["len_kept"], -1]
+        s = np.asarray(s, dtype=np.int32)
+        _lib.check(self.lib.deepj_cuda_flush_ops_async(s.ctypes.data, s.size))
+        self._evicted = True
+        self._rows = kept
+        self._upload(I["len"], kept)
 
     def prefill_packed(self, prompts) -> np.ndarray:
         """Feed prompts of different lengths, one per sequence (each at least one token), behind whatever the sequences hold; returns the greedy

@@ -6,7 +6,7 @@ from deepj_b200 import compute_graph as cg
 from deepj_b200.decoder import DecoderConfig, Q8Decoder
 from q4_standin import box, standin  # noqa: F401
 
-CFG = DecoderConfig("gpt", 64, 96, 64, 2, 1, 96)
+CFG = DecoderConfig("gpt", 64, 200, 64, 2, 1, 96)
 
 
 @pytest.fixture
@@ -109,3 +109,41 @@ class Failing:
 
     def __getattr__(self, name):
         return getattr(self._real, name)
+
+
+def evictions(box):  # noqa: F811
+    """(sequence, rows it had) of the sequences that the last launches evicted from; one layer."""
+    return [(b, n) for kind, b, n, budget in box.launched() if kind == cg.OP_KV_EVICT_Q4 and n > budget]
+
+
+def test_only_full_sequences_are_evicted_from(make, box):  # noqa: F811
+    d = make(3, kv_rows=64, kv_budget=40)
+    d.prefill_packed([[1] * 15, [2] * 1, [3] * 24])
+    d.prefill_packed([[1] * 24, [2] * 24, [3] * 24])
+    d.prefill_packed([[1] * 24, [2] * 20, [3] * 1])
+    assert state(d)[0] == [63, 45, 49]
+    box.launched()
+    d.step([1, 2, 3])
+    assert evictions(box) == [] and state(d)[:2] == ([64, 46, 50],) * 2
+    d.step([1, 2, 3])
+    assert evictions(box) == [(0, 64)] and state(d) == ([41, 47, 51], [41, 47, 51], [65, 47, 51])
+    d.prefill_packed([[1] * 2, [2] * 20, [3] * 1])
+    assert evictions(box) == [(1, 47)] and state(d)[:2] == ([43, 60, 52],) * 2
+    d.prefill([[1] * 10] * 3, chunked=True)                          # fits the first; the others make room
+    assert evictions(box) == [(1, 60)] and state(d)[:2] == ([53, 50, 62],) * 2
+    d.prefill_packed([[1] * 1, [2] * 30, [3] * 25])                  # passes of 24: the first one's prompt has ended by the second
+    assert evictions(box) == [(1, 50), (2, 62), (1, 64), (2, 64)] and state(d)[:2] == ([54, 46, 41],) * 2
+    d.step_device(24)
+    assert evictions(box) == [(0, 64), (1, 64), (2, 64)] and state(d)[0] == [54, 46, 41]
+    with pytest.raises(ValueError, match="evicted"):
+        d.set_position(20)
+
+
+def test_a_refused_chunk_evicts_nothing(make, box):  # noqa: F811
+    d = make(2, kv_rows=64, kv_budget=40)
+    d.prefill_packed([[1] * 24, [2] * 24])
+    d.prefill_packed([[1] * 24, [2] * 1])
+    box.launched()
+    with pytest.raises(ValueError, match="more tokens"):
+        d._make_room(30)
+    assert evictions(box) == [] and state(d)[:2] == ([48, 25],) * 2
