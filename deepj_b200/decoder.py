@@ -644,11 +644,20 @@ class Q8Decoder(StreamDecoder):
         self._upload(self.ids["len"], rows.astype(np.float32))
 
     _evicted = False         # cached rows are no longer the first positions
+    _timed_seen: Optional[int] = None
 
     def _check_room(self, tokens) -> None:
         """Refuses `tokens` new rows (of every sequence, or one number each) that a 4-bit cache without a budget has no room for."""
         if self.kv_dtype == "q4" and self.kv_budget is None and np.any(self._rows + tokens > self.kv_rows):
             raise ValueError(f"the cache holds {self.kv_rows} rows per sequence and has no budget to evict to")
+
+    def _repeatable(self, op: np.ndarray) -> np.ndarray:
+        if op[0] == OP_ATTN_DECODE_Q4 and op[19] >= 0:                   # weights are added up in place: to a buffer of their own here
+            if self._timed_seen is None:
+                self._timed_seen = self._f32("", self.B * self.h_local * self.kv_rows)
+            op = op.copy()
+            op[19] = self._timed_seen
+        return op
 
     def _advance(self, tokens) -> None:
         super()._advance(int(np.max(tokens)))

@@ -79,6 +79,10 @@ class StreamDecoder:
     def _make_room(self, tokens: int) -> None:
         """Called before `tokens` new tokens of every sequence run: a cache that is full makes room here."""
 
+    def _repeatable(self, op: np.ndarray) -> np.ndarray:
+        """An op's words for a stream that is run again and again for its time: as they are, unless a repeat would change what later steps do."""
+        return op
+
     def _advance(self, tokens: int) -> None:
         """Counts `tokens` tokens of every sequence, which have been enqueued."""
         self.position += tokens
@@ -377,7 +381,7 @@ class StreamDecoder:
         """Device time of the ops whose label is in `labels`, run back to back as their own stream
         (graph-replayed like the full step, at the current position): (ms per pass, ops per pass)."""
         full = self._build(feed_back=False)
-        keep = [full[a:b] for lbl, (a, b) in zip(self._op_labels, self._op_bounds) if lbl in labels]
+        keep = [self._repeatable(full[a:b]) for lbl, (a, b) in zip(self._op_labels, self._op_bounds) if lbl in labels]
         if not keep:
             return 0.0, 0
         sub = np.ascontiguousarray(np.concatenate(keep))

@@ -81,7 +81,10 @@ size_t q4_decode_ws_floats(const Q4AttnArgs&) { return 0; }
 size_t q4_evict_ws_floats(const Q4EvictArgs&) { return 0; }
 void launch_q4_append(const Q4AttnArgs& a, int T, cudaStream_t) { note(90, a.M, T); }
 void launch_q4_attn(const Q4AttnArgs& a, cudaStream_t) { if (a.M > 0 || a.accOut != nullptr) note(88, a.M, a.H, a.G); }
-void launch_q4_decode(const Q4AttnArgs& a, cudaStream_t) { note(87, a.early, a.H, a.G); }
+void launch_q4_decode(const Q4AttnArgs& a, cudaStream_t) {
+    if (a.accOut != nullptr) a.accOut[0] = a.acc[0] + 1.0f;          // weights are added up
+    note(87, a.early, a.H, a.G);
+}
 void launch_q4_load(const Q4LoadArgs& a, cudaStream_t) { if (a.T > 0) note(91, a.T); }
 void launch_q4_evict(const Q4EvictArgs& a, cudaStream_t) {
     for (int b = 0; b < a.B; b++) {

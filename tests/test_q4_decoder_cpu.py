@@ -147,3 +147,14 @@ def test_a_refused_chunk_evicts_nothing(make, box):  # noqa: F811
     with pytest.raises(ValueError, match="more tokens"):
         d._make_room(30)
     assert evictions(box) == [] and state(d)[:2] == ([48, 25],) * 2
+
+
+def test_timing_leaves_what_decides_evictions(make):
+    d = make(2, kv_rows=64, kv_budget=40)
+    d.prefill_packed([[1] * 5, [2] * 3])
+    d.step([1, 2])
+    before = d._download(d.ids["seen.0"], 2 * 2 * 64)
+    assert before[0] == 1.0 and d.time_ops({"attn"}, iters=4)[1] == 1
+    assert np.array_equal(d._download(d.ids["seen.0"], 2 * 2 * 64), before) and state(d)[0] == [6, 4]
+    d.step([1, 2])
+    assert d._download(d.ids["seen.0"], 1)[0] == 2.0
