@@ -2,11 +2,12 @@
 //
 // A warp streams pages of 32 rows through a ring of its own, one bulk copy each, and keeps the running maximum and sum of the softmax in fp32.  Both
 // products run on the integer tensor pipe, exactly:
-//   scores   A = 16 rows × 32 dims of int8 codes (a masked page word is an operand register), B = the query in fixed point, 23 bits of its largest
-//            value, as three signed base-256 digits.  A 32-dim block's integer sums are multiplied by the row's scale in fp32.
+//   scores   A = 16 rows × 32 dims of int8 codes (a masked page word is an operand register), B = the query in fixed point, 31 bits of its largest
+//            value, as four signed base-256 digits.  A 32-dim block's integer sums are multiplied by the row's scale in fp32.
 //   values   A = 16 dims × 32 rows (a byte transpose of four rows' words), B = weight × scale of the row and block, in fixed point of the page's
 //            largest such product, three digits again.
-// Columns 2t and 2t + 1 of B are digit t of two heads, so a lane sees one digit of up to two heads per tile and the digits meet in shuffles.
+// Columns 2t and 2t + 1 of B are digit t of two heads, so a lane sees one digit of up to two heads per tile and the digits meet in shuffles.  (With three digits of
+// the query, which leaves two columns empty, one value of 2^12 times the others cost these all but ten bits, also where no key had anything there.)
 // The new row is quantized by the warp that holds its page, into the page's copy in shared memory and into the cache: later steps read what this one did.
 //
 // Few heads: a cluster of up to eight blocks shares a sequence and head and exchanges maxima, sums and unnormalised rows through distributed shared
@@ -85,7 +86,7 @@ template <int NB, int HPB> struct DecodeShape {
     static constexpr int kStages = NB == 4 ? 2 : NB == 2 ? 3 : 6;
     static constexpr int kRing = kStages * Q4Page<NB>::kBytes;           // of a warp
     static constexpr int kDigits = NB * HPB * 96;                        // … [block][head][digit][32 rows]
-    static constexpr int kQuery = HPB * 3 * HD;                          // … the queries' digits
+    static constexpr int kQuery = HPB * 4 * HD;                          // … the queries' digits
     static constexpr int kWarp = kRing + kDigits + kQuery;
     static constexpr size_t kSmem = kDecWarps * kWarp + 64;              // 64: zeros for the columns without a head
     // blocks of an SM: the stream's registers want room (16 sequences of 32 heads of 128: 37 µs with four, 41 with five); blocks that are many and short want
@@ -150,30 +151,33 @@ struct DecodeWarp {
         float back, bad = fmaf(q.x, 0.0f, fmaf(q.y, 0.0f, fmaf(q.z, 0.0f, q.w * 0.0f)));
         const float mul = fixed_of(warp_max(fmaxf(fmaxf(fabsf(q.x), fabsf(q.y)), fmaxf(fabsf(q.z), fabsf(q.w)))), back);
         bad = __any_sync(0xffffffffu, bad != bad) ? __int_as_float(0x7fc00000) : 0.0f;      // NaN where the query holds an infinity or a NaN
-        const uint32_t u0 = digits_of(q.x, mul), u1 = digits_of(q.y, mul), u2 = digits_of(q.z, mul), u3 = digits_of(q.w, mul);
+        auto digits4 = [&](float x) { return ((uint32_t)__float2int_rn(x * mul * 256.0f) + 0x808080u) ^ 0x808080u; };      // below 2^30
+        const uint32_t u0 = digits4(q.x), u1 = digits4(q.y), u2 = digits4(q.z), u3 = digits4(q.w);
         const uint32_t t0 = __byte_perm(u0, u1, 0x5140), t1 = __byte_perm(u2, u3, 0x5140), t2 = __byte_perm(u0, u1, 0x7362), t3 = __byte_perm(u2, u3, 0x7362);
         if (lane < LPR) {
-            to[2 * (HD / 4) + e] = __byte_perm(t0, t1, 0x5410);
-            to[HD / 4 + e] = __byte_perm(t0, t1, 0x7632);
-            to[e] = __byte_perm(t2, t3, 0x5410);
+            to[3 * (HD / 4) + e] = __byte_perm(t0, t1, 0x5410);
+            to[2 * (HD / 4) + e] = __byte_perm(t0, t1, 0x7632);
+            to[HD / 4 + e] = __byte_perm(t2, t3, 0x5410);
+            to[e] = __byte_perm(t2, t3, 0x7632);
         }
         return back * p.scale * (1.0f / 16.0f) + bad;
     }
-    __device__ __forceinline__ float digit() const { return t == 0 ? 65536.0f : t == 1 ? 256.0f : t == 2 ? 1.0f : 0.0f; }      // what this lane's digit counts for
+    __device__ __forceinline__ float digit() const { return t == 0 ? 65536.0f : t == 1 ? 256.0f : t == 2 ? 1.0f : 0.0f; }      // what this lane's digit of a weight counts for
+    __device__ __forceinline__ float query_digit() const { return t == 3 ? 1.0f / 256.0f : digit(); }
     // Operands from all heads' digits; an empty softmax.
     __device__ __forceinline__ void begin(const uint32_t* queries, const float* factors) {
         const int hc = g & 1, dc = g >> 1;        // head and digit of the B column this lane fills
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const bool on = dc < 3 && 2 * n + hc < HPB;
-            const uint32_t* const from = queries + (on ? ((2 * n + hc) * 3 + dc) * (HD / 4) : 0);
+            const bool on = 2 * n + hc < HPB;
+            const uint32_t* const from = queries + (on ? ((2 * n + hc) * 4 + dc) * (HD / 4) : 0);
 #pragma unroll
             for (int j = 0; j < NB; j++) {
                 bq[n][j][0] = on ? from[8 * j + t] : 0;
                 bq[n][j][1] = on ? from[8 * j + 4 + t] : 0;
             }
 #pragma unroll
-            for (int c = 0; c < CH; c++) factor[n][c] = factors[2 * n + c] * digit();
+            for (int c = 0; c < CH; c++) factor[n][c] = factors[2 * n + c] * query_digit();
 #pragma unroll
             for (int j = 0; j < NB; j++)
 #pragma unroll
@@ -330,7 +334,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kShort) 
     constexpr int HD = S::HD, kOut = HPB * HD, W = kDecWarps;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) unsigned long long s_bar[W * S::kStages];
-    __shared__ __align__(16) uint32_t s_q[HPB * 3 * HD / 4];
+    __shared__ __align__(16) uint32_t s_q[HPB * 4 * HD / 4];
     __shared__ float s_factor[HPB], s_m[W][HPB], s_l[W][HPB], s_own[HPB][2];
     __shared__ float s_ml[CLUSTER ? kDecCluster : 1][HPB][2];            // every split's maximum and sum
     __shared__ float s_red[CLUSTER ? kOut : 1];                          // this block's share of the output row, of every split
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kShort) 
     const size_t tab = (size_t)pos * (HD / 2) + 2 * w.e;
     const float2 cs = *reinterpret_cast<const float2*>(p.cosT + tab), sn = *reinterpret_cast<const float2*>(p.sinT + tab);
     if (warp < HPB) {
-        const float f = w.put_query(s_q + warp * 3 * (HD / 4), q, cs, sn);
+        const float f = w.put_query(s_q + warp * 4 * (HD / 4), q, cs, sn);
         if (w.lane == 0) s_factor[warp] = f;
     }
     __syncthreads();
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecodeShape<NB, HPB>::kResiden
         for (int h = 0; h < HPB; h++) q[h] = h < heads ? *reinterpret_cast<const float4*>(row + p.q_off + (h0 + h) * HD + 4 * w.e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int h = 0; h < HPB; h++) {
-            const float f = w.put_query(w.query + h * 3 * (HD / 4), q[h], cs, sn);
+            const float f = w.put_query(w.query + h * 4 * (HD / 4), q[h], cs, sn);
             if (lane == 0) s_factor[warp][h] = f;
         }
         __syncwarp();

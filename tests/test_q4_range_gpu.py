@@ -130,3 +130,34 @@ def test_scores_of_any_size_choose_a_key(dev, packed, hd, G, n, scale):  # noqa:
             if gap < 30.0 + 4 * 2.0 ** -21 * A:                      # two keys the operands' 22 bits do not tell apart
                 continue
             assert np.all(np.abs(got[t, g] - v[order[-1]]) <= 2.0 ** -20 * np.abs(v).max()), (t, g, got[t, g][:4], v[order[-1]][:4])
+
+
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("channel", [5, 70])
+@pytest.mark.parametrize("G,R,n", [(2, 1, 200), (1, 4, 900), (1, 1, 9000)])
+def test_queries_with_one_large_value(dev, packed, channel, G, R, n):  # noqa: F811
+    """One value of each query is 2^12 times the others, and no key has anything there: the scores are the other values' alone.  Operands of 30 bits and more of the
+    largest value (steps: half a step is 2^-30 of it, prompts: 2^-33) hold these to 18."""
+    hd, M = 128, 4 if packed else 1
+    rng = np.random.default_rng(channel + n)
+    K, V, q, k_new, v_new = rows(rng, G, n, hd), rows(rng, G, n, hd), rng.standard_normal((M, G * R, hd)).astype(np.float32), rows(rng, M, G, hd), rows(rng, M, G, hd)
+    K[..., channel], k_new[..., channel], q[..., channel] = 0.0, 0.0, 4096.0 * np.abs(q).max()
+    got, weights = attend(dev, K, V, np.concatenate((q, k_new, v_new), 1).reshape(M, -1), n, packed, R, window=M)
+    k_new, v_new = ref.stored(k_new).astype(np.float64), ref.stored(v_new).astype(np.float64)
+    want_w, tol_w = np.zeros((G, n + M)), np.zeros((G, n + M))
+    for t in range(M):
+        for h in range(G * R):
+            g = h // R
+            k = np.concatenate((ref.stored(K[g]).astype(np.float64), k_new[:t + 1, g]))
+            v = np.concatenate((ref.stored(V[g]).astype(np.float64), v_new[:t + 1, g]))
+            x = q[t, h].astype(np.float64)
+            sc = k @ x / np.sqrt(hd)
+            off = 2.0 ** -30 * np.abs(x).max() * np.abs(k).sum(1).max() / np.sqrt(hd) + 2.0 ** -21 * (np.abs(k) @ np.abs(x) / np.sqrt(hd)).max()
+            p = np.exp(sc - sc.max())
+            p /= p.sum()
+            rel = 2 * off + 2.0 ** -19                               # the sums of weights among it, as above
+            assert np.all(np.abs(got[t, h] - p @ v) <= rel * np.abs(v).max())
+            want_w[g, :n + t + 1] += p
+            tol_w[g, :n + t + 1] += rel * p
+    err = np.abs(weights - want_w) / tol_w
+    assert np.all(err <= 1.0), float(err.max())
