@@ -10,8 +10,8 @@ namespace {
 
 // ───────────── rows in ─────────────
 // Row m of the source is token t of sequence b: m = b·T + t, or (starts) the packed row that lies in starts[b] … starts[b + 1].  A row of a head is
-// 4·NB lanes of eight values, a word of the page each.  The bytes are 8·hd read and 1.125·hd written per row and head; what bounds it is the instructions
-// for the codes (2048 rows of 32 heads of 128: 20 µs where the bytes take 12; with four values to a lane 27).
+// 4·NB lanes of eight values, a word of the page each.  The bytes are 8·hd read and 1.125·hd written per row and head.  2048 rows of 32 heads of 128: 20 µs where
+// the bytes take 12 (with four values to a lane 27); no unit is at its limit (64 % of the issue slots, ALU 48 %): the loads' latency and the instructions for the codes.
 struct AppendParams {
     const float* src; int k_off, v_off, ld;
     unsigned char* cache; int maxSeq, pages;

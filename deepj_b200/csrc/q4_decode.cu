@@ -14,9 +14,11 @@
 // memory.  Many: all pages of all sequences and heads in a row are dealt out evenly to the warps of a grid that fills the chip once (k_q4_stream).  A warp
 // writes the output of a head whose pages it has all seen; of the first and the last one, which it may share with its neighbours, it leaves a record for
 // k_q4_finish.  One block per head instead, 16 sequences of 1024 … 2048 rows and 32 heads: 46 µs with a third of the chip idle at the end.
-// Weights are added up from the scores, which wait in the workspace until a row's maximum and sum are known.
-// Bound by instructions (600 … 900 a page and warp): 16 sequences of 1024 … 2048 rows and 32 heads of 128 with weights 38 µs, 4.1 TB/s of the cache's bytes while
-// the stream runs; 4 of 32700 and 32/8 heads 62 µs.  Small steps by the launch and a page's latency: one sequence of 2048, 32 heads 10 µs.
+// Weights are added up from the scores, which wait in the workspace until a row's maximum and sum are known: B · H · (rows of the cache, whatever the lengths)
+// floats.
+// 16 sequences of 1024 … 2048 rows and 32 heads of 128 with weights: 38.8 µs, 4.2 TB/s of the cache's bytes while the stream runs; 4 of 32700 and 32/8 heads
+// 62 µs.  No unit is at its limit there (57 and 62 % of the issue slots, ALU 46 %): the latency of a page's chain of some 600 … 900 instructions, with the 16 and
+// 12 warps that an SM has registers for.  Small steps are the launch and a page's latency: one sequence of 2048, 32 heads 10.2 µs.
 #include <algorithm>
 #include <cmath>
 
@@ -90,7 +92,8 @@ template <int NB, int HPB> struct DecodeShape {
     static constexpr int kWarp = kRing + kDigits + kQuery;
     static constexpr size_t kSmem = kDecWarps * kWarp + 64;              // 64: zeros for the columns without a head
     // blocks of an SM: the stream's registers want room (16 sequences of 32 heads of 128: 37 µs with four, 41 with five); blocks that are many and short want
-    // places (64 sequences of 12 heads of 64: 14.4 with four, 12.3 with five, 10.3 with six), unless that spills (32 of 16 heads of 128: 10.3 and, with five, 12.3)
+    // places (64 sequences of 12 heads of 64, back to back on one input: 14.4 with four, 12.3 with five, 10.3 with six), unless that spills (32 of 16 heads of
+    // 128: 10.3 and, with five, 12.3)
     static constexpr int kResident = HPB == 4 ? 3 : 4, kShort = HPB == 1 && NB < 4 ? 6 : kResident;
 };
 
@@ -756,8 +759,9 @@ DecodePlan decode_plan(const Q4AttnArgs& a) {
     d.pages = (a.maxSeq + kQ4Page - 1) / kQ4Page;
     d.blocks = (d.perBlock == 4 ? 3 : 4) * g_num_sms;                    // all that are resident at once
     const long long heads = (long long)a.B * a.G * d.headBlocks;
-    // Clusters of up to eight where they fit onto the chip together, until a warp has a page (16 heads of 10 pages: 5.5 µs with two blocks to a head, 4.8 with four).  Pages in a row where a block would have more than 32 of a head (16 sequences of
-    // 32 heads with 65 each 46 µs a block each, 41 in a row; 64 of 12 heads with 7 each 15 and 18.5).
+    // Clusters of up to eight where they fit onto the chip together, until a warp has a page (16 heads of 10 pages: 5.5 µs with two blocks to a head, 4.8 with
+    // four).  Pages in a row where a block would have more than 32 of a head (16 sequences of 32 heads with 65 each 46 µs a block each, 41 in a row; 64 of 12
+    // heads with 7 each 15 and 18.5).
     d.splits = 1;
     while (d.splits < kDecCluster && d.splits * kDecWarps < d.pages && heads * d.splits * 2 <= d.blocks) d.splits *= 2;
     d.stream = d.pages > 8 * kDecWarps * d.splits || (a.accOut != nullptr && d.headBlocks > 1);

@@ -14,8 +14,8 @@
 // share an SM (half of its tensor and shared memory each: two S/P buffers of 64 columns, O, one tile of keys and one of values).  One block per SM with
 // tiles of 128 keys and two of each took 3900 cycles for 128 keys, where the MMAs take 2048.
 // Where tiles of queries are few, up to four blocks (a cluster) share the keys of one and join their outputs through shared memory, a part of the rows each.
-// Measured: 2048 tokens of 32 heads of 128 88 µs (780 TFLOP/s counting the halves), 6000 of 32/8 heads 510 µs (1150); bound by the chain of a tile (2900 cycles with two
-// blocks on an SM) and by what a block does before its first and after its last tile (25000 cycles).
+// Measured: 2048 tokens of 32 heads of 128 86 µs (800 TFLOP/s counting the halves; 101 µs with cold caches), 6000 of 32/8 heads 510 µs (1150).  Bound by the chain
+// of a tile (2900 cycles with two blocks on an SM) and by what a block does before its first and after its last tile (25000 cycles).
 // Every wait is bounded (codes 341-350 in the device error word).
 #include <algorithm>
 #include <cmath>
@@ -45,15 +45,15 @@ struct PrefillParams {
 };
 constexpr int kMaxSplits = 4;
 // Tiles whose values are summed in tensor memory.  Those sums are cut off, not rounded: values of one sign lose 5.6e-9 of their sum a key, 3.4e-5 at 6000 keys.
-// So a sum of 16 tiles goes to memory, where it is added rounded: 6e-6 at any length (32 tiles: 1.1e-5), for 3 % of the time at 1500 keys and 6 % at 6000
-// (emptied every 8 tiles: 12 % and 14 %).  The sums of the weights go the same way, a tile's and then sixteen tiles' by themselves: a chain of 16 thousand
-// equal weights was off by 2e-4.
+// So a sum of 16 tiles goes to memory, where it is added rounded: 5e-6 from 4000 to 65000 keys (32 tiles: 1.1e-5), for 3 % of the time at 1500 keys and 6 % at
+// 6000.  For values of both signs, 6000 tokens of 32/8 heads: 1.8e-6, with 10 tiles 1.3e-6 and 5 % more time, with 8 1.2e-6 and 8 %, plain fp32 0.8e-6.
+// The sums of the weights go the same way, a tile's and then sixteen tiles' by themselves: a chain of 16 thousand equal weights was off by 1e-4.
 constexpr int kSegment = 16;
 // A row's weights are taken to a base 2^9 below its maximum, P up to 2^9, and the base stays until one would be above 2^15, the last power of two in fp16.  Steps of
 // fp16 end at 2^-24: with the maximum at 2^9, a weight is off by at most 2^-33 of the row's largest (two halves, half a step each).  With the maximum at 1, weights under
 // 2^-14 of it kept 10 bits and fewer, those under 2^-25 none: thousands of keys 10 … 18 nats below one were off by up to all of their sum.
 constexpr float kLift = 9.0f, kTop = 15.0f;
-// The base for a maximum; scores beyond 2^26 have no places for the lift, and a step of theirs may be more than it.
+// The base for a maximum; from 2^27 on a step of a score is more than the lift.
 __device__ __forceinline__ float base_of(float most) { return most - (most - kLift) > kTop ? most : most - kLift; }
 
 constexpr size_t kAlone = 120 * 1024;             // more than half of an SM's shared memory
@@ -164,9 +164,9 @@ __device__ __forceinline__ void zero_row(unsigned char* tile, int row, int t0, i
 // Query rows of a tile, rotated, in halves of fp16 times a power of two → tiles hi and lo, a row to 4·NB lanes of eight values each, one 16-byte piece;
 // `place(row, m, head, position)` says which one row `row` of the first `rows` is, and whether it is one (false: zeros, but the place can be read).
 // factors[row] makes a sum of products a score in log2 units (NaN where the row holds an infinity or a NaN).  It is a power of two, 1/sqrt(hd) · log2(e) goes
-// into the values: a score is then exact, and the one that its row's base was taken from comes to the lift again, however large scores are.  Bound by instructions: four values to a lane
-// took 12000 cycles a tile of four heads a token, eight 9000.  Loads of several rows ahead cost more in code than they give: the roles of a block share
-// the instruction cache (eight prompts of 1500: 303 µs as it is, 307 and 319 with two and three rows ahead).
+// into the values: a score is then exact, and the one that its row's base was taken from comes to the lift again, however large scores are.
+// Four values to a lane took 12000 cycles a tile of four heads a token, eight 9000.  Loads of several rows ahead cost more in code than they give: the roles
+// of a block share the instruction cache (eight prompts of 1500: 303 µs as it is, 307 and 319 with two and three rows ahead).
 template <int NB, typename Place>
 __device__ __forceinline__ void query_rows(const PrefillParams& p, int warp, int warps, int lane, unsigned char* hi, unsigned char* lo, float* factors, int rows, Place place) {
     constexpr int HD = 32 * NB, LPR = 4 * NB, RPW = 32 / LPR;
@@ -559,8 +559,9 @@ __global__ void __launch_bounds__(kPThreads, 2) k_q4_prefill(const PrefillParams
                 asked = j + 1;                    // everything of this tile is in registers
                 if (lane == 0 && j + 1 < tiles && 2 * (j + 1) + (w >> 1) < pages) {
                     mbar_arrive_expect_tx(arrived, S::kRaw);
-                    bulk_g2s(smem_u32(raw_at), from + (size_t)(j + 1) * (2 * Q4Page<NB>::kBytes), 16 * Q4Page<NB>::kRow, arrived);
-                    bulk_g2s(smem_u32(raw_at) + 16 * Q4Page<NB>::kRow, from + (size_t)(j + 1) * (2 * Q4Page<NB>::kBytes) + Q4Page<NB>::kKs - (w & 1) * (16 * Q4Page<NB>::kRow - 32 * NB), 32 * NB, arrived);
+                    const unsigned char* const next = from + (size_t)(j + 1) * (2 * Q4Page<NB>::kBytes);
+                    bulk_g2s(smem_u32(raw_at), next, 16 * Q4Page<NB>::kRow, arrived);
+                    bulk_g2s(smem_u32(raw_at) + 16 * Q4Page<NB>::kRow, next + Q4Page<NB>::kKs - (w & 1) * (16 * Q4Page<NB>::kRow - 32 * NB), 32 * NB, arrived);
                 }
             }
             if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait_long(value ? vEmpty : kEmpty, (j - 1) & 1, &s_abort, p.error, 344))) break;

@@ -311,13 +311,15 @@ int deepj_cuda_latent_alloc(int32_t id, int32_t batch, int32_t max_seq, int32_t 
  *
  * Ops over a 4-bit cache (deepj_cuda_kv_alloc_q4), H query heads over its G key/value heads, H a multiple of G.  A sequence whose length is
  * outside 0 … max_seq - 1 or whose position is outside 0 … max_pos - 1 (NaN is) is left out: nothing of it is appended or written.  Tokens that
- * do not fit (behind max_seq rows or max_pos positions) are left out as well, rows outside 0 … M - 1 are none of a sequence's.  Offsets and strides are multiples of four floats.
- * An output is another buffer than the inputs and the other outputs; where it says so below, weights may be added up in place.
+ * do not fit (behind max_seq rows or max_pos positions) are left out as well, rows outside 0 … M - 1 are none of a sequence's.  A query that holds an
+ * infinity or a NaN gives NaN.  Offsets and strides are multiples of four floats.  An output is another buffer than the inputs and the other outputs;
+ * where it says so below, weights may be added up in place.
  *
  *  87 ATTN_DECODE_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, acc, acc_out]
  *                        one token of every sequence: q and k rotated at pos[b] (tables [max_pos][hd/2]), k and v appended as row len[b], softmax
  *                        attention over rows 0..len[b].  acc, acc_out [B][G][max_seq] (or both -1; may be one buffer): acc_out of row j =
- *                        (j < len[b] ? acc : 0) + the softmax weights that the G's query heads give row j; entries beyond len[b] stay
+ *                        (j < len[b] ? acc : 0) + the softmax weights that the G's query heads give row j; entries beyond len[b] stay.
+ *                        With weights the workspace ([4] of deepj_cuda_stats) holds B * H * max_seq floats, whatever the lengths
  *  88 ATTN_PACKED_Q4    [op, qkv, q_off, k_off, v_off, ld, kv, layer, starts, len, pos, cos, sin, max_pos, out, out_off, ldo, B, H, M, acc, acc_out, window]
  *                        prompts of different lengths: rows starts[b] .. starts[b+1]-1 of the M rows are the tokens of sequence b (none is fine; rows
  *                        of no sequence stay as they are; ranges must not overlap).  Token t is rotated at pos[b] + t, appended as row len[b] + t and
