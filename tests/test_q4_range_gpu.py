@@ -161,3 +161,21 @@ def test_queries_with_one_large_value(dev, packed, channel, G, R, n):  # noqa: F
             tol_w[g, :n + t + 1] += rel * p
     err = np.abs(weights - want_w) / tol_w
     assert np.all(err <= 1.0), float(err.max())
+
+
+@pytest.mark.parametrize("R,M", [(1, 3000), (8, 2000), (33, 300)])
+def test_weights_of_many_tokens_add_up(dev, R, M):  # noqa: F811
+    """All weights of a token are equal, one over its keys: an old row gets a sum of R · M of them, whose roundings all go the same way for long stretches."""
+    hd, n = 32, 5
+    qkv = np.zeros((M, (R + 2) * hd), np.float32)
+    qkv[:, (R + 1) * hd:] = 7.0
+    K = np.full((1, n, hd), 7.0, np.float32)                         # stored as they are
+    got, weights = attend(dev, K, K, qkv, n, True, R, window=M)
+    each = R / (n + 1.0 + np.arange(M))
+    tail = np.cumsum(each[::-1])[::-1]
+    want = np.concatenate((np.full(n, tail[0]), tail))
+    # exponential and quotient 2^-20; additions one behind the other, half a step each: a token's sum 64, then 64 of a tile of 128 query rows, and the tiles
+    rel = 2.0 ** -20 + (64 + 64 + (R * M + 127) // 128) * 2.0 ** -25
+    err = np.abs(weights[0] / want - 1.0).max()
+    assert err <= rel, (float(err), rel)
+    assert np.all(np.abs(got / 7.0 - 1.0) <= relative(0.0))
